@@ -13,6 +13,7 @@ SPACES = {"l2": 0, "cosine": 1, "ip": 2}
 SHADOWS = {"none": 0, "bf16": 1, "i8": 2, "auto": 3}
 MODE_AUTO, MODE_EXACT, MODE_MFMA = 0, 1, 2
 MAX_K = 128
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "tanh": 5}
 PAD_KEY = 0xFFFFFFFFFFFFFFFF
 
 EXPORTS = [
@@ -40,6 +41,10 @@ EXPORTS = [
     "hrs_encoder_load",
     "hrs_encoder_release",
     "hrs_encode",
+    "hrs_linear",
+    "hrs_attention",
+    "hrs_attention_workspace",
+    "hrs_layer_norm",
     "hrs_row_mask_update",
     "hrs_postings_register",
     "hrs_postings_release",
@@ -63,6 +68,18 @@ EXPORTS = [
 
 class EncoderConfigC(C.Structure):
     _fields_ = [("vocab", C.c_int), ("hidden", C.c_int), ("layers", C.c_int), ("heads", C.c_int), ("inter", C.c_int), ("max_pos", C.c_int), ("eps", C.c_float)]
+
+
+class AttentionArgsC(C.Structure):
+    _fields_ = (
+        [(n, C.c_void_p) for n in ("q", "k", "v", "out")]
+        + [(n, C.c_int) for n in ("dtype", "batch", "q_heads", "kv_heads", "head_dim", "causal")]
+        + [("scale", C.c_float), ("softcap", C.c_float), ("bias_reach", C.c_int)]
+        + [(n, C.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride")]
+        + [("q_rows", C.c_int64), ("k_rows", C.c_int64)]
+        + [(n, C.c_void_p) for n in ("q_offs", "k_offs", "q_lens", "k_lens", "prefix_lens", "slopes", "bias_table")]
+        + [("max_q", C.c_int64), ("max_k", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+    )
 
 
 class HrsError(RuntimeError):
@@ -108,6 +125,10 @@ def lib():
             "hrs_encoder_load": ([vp, vp, vp, vp, C.POINTER(vp)], i32),
             "hrs_encoder_release": ([vp, vp], i32),
             "hrs_encode": ([vp, vp, vp, vp, i32, i32, vp, vp], i32),
+            "hrs_linear": ([vp, i32, vp, i64, vp, i64, vp, vp, i64, i32, vp, i64, i64, i64, i64, vp], i32),
+            "hrs_attention": ([vp, vp, vp], i32),
+            "hrs_attention_workspace": ([vp, vp, C.POINTER(C.c_size_t)], i32),
+            "hrs_layer_norm": ([vp, i32, vp, i64, vp, i64, vp, vp, C.c_float, vp, i64, i64, i64, vp], i32),
             "hrs_row_mask_update": ([vp, i64, vp, vp, i32, i32, vp, i32, vp, vp], i32),
             "hrs_postings_register": ([vp, vp, vp, i64, i64, C.POINTER(vp)], i32),
             "hrs_postings_release": ([vp, vp], i32),

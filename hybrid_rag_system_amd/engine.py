@@ -20,6 +20,9 @@ def _stream():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # hrs_type
+
+
 class Corpus:
     """The embedding matrix of one shard, registered with the engine (keeps `matrix` alive)."""
 
@@ -446,6 +449,171 @@ class Engine:
         counts = self.keyword_counts(postings, q_terms, q_term_offs, rows)
         combined, perm = self.fuse_sort(dist, counts, q_term_offs, n, boost)
         return {"cand_dist": dist, "cand_rows": rows, "cand_counts": counts, "combined": combined, "perm": perm}
+
+    # ---- operators of an encoder layer ----------------------------------------------------------
+    def _check(self, name, t, dtype, shape=None):
+        """A tensor of this GPU, of one type, and of one shape where the others fix it."""
+        if not (t.is_cuda and t.device == self.device):
+            raise ValueError(f"{name} must be on {self.device}, not on {t.device}")
+        if t.dtype != dtype:
+            raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
+        if shape is not None and tuple(t.shape) != shape:
+            raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {shape}")
+
+    def _rows(self, name, t, dtype, n=None):
+        """[.., N] with its elements next to each other as rows: -> the [rows, N] view (no copy)."""
+        self._check(name, t, dtype)
+        if t.dim() < 1 or (n is not None and t.shape[-1] != n):
+            raise ValueError(f"{name}: shape {tuple(t.shape)}, expected [.., {n}]")
+        if t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError(f"{name}: the elements of a row must be next to each other (last stride {t.stride(-1)})")
+        if t.dim() == 2:
+            return t
+        try:
+            return t.view(-1, t.shape[-1]) if t.numel() else t.reshape(-1, t.shape[-1]) if t.shape[-1] else t.new_empty((t.shape[:-1].numel(), 0))
+        except RuntimeError:
+            raise ValueError(f"{name}: rows at strides {tuple(t.stride())} have no common stride") from None
+
+    def _vector(self, name, t, n):
+        if t is None:
+            return None
+        self._check(name, t, torch.float32, (n,))
+        if n > 1 and t.stride(0) != 1:
+            raise ValueError(f"{name} must be contiguous")
+        return t.data_ptr()
+
+    def _queue(self):
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def linear(self, x, weight, bias=None, activation="none", residual=None, out=None):
+        """act(x @ weight.T + bias) + residual in one kernel (hrs_linear): x [.., K] and weight [N, K] bf16 or fp16, bias
+        fp32 [N], residual [.., N] as x; activation "none", "relu", "gelu" (erf), "gelu_tanh", "silu" or "tanh".  Rows may
+        lie at any stride.  Sums, bias, activation and residual in fp32, one rounding.  out (as the result) may be
+        residual, not x or weight."""
+        if x.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"x must be bfloat16 or float16, not {x.dtype}")
+        if activation not in N.ACTIVATIONS:
+            raise ValueError(f"unknown activation {activation!r}: one of {', '.join(N.ACTIVATIONS)}")
+        if weight.dim() != 2:
+            raise ValueError(f"weight: shape {tuple(weight.shape)}, expected [N, K]")
+        n, k = weight.shape
+        x2, w = self._rows("x", x, x.dtype, k), self._rows("weight", weight, x.dtype)
+        shape = x.shape[:-1] + (n,)
+        m = x2.shape[0]
+        r = None
+        if residual is not None:
+            self._check("residual", residual, x.dtype, tuple(shape))
+            r = self._rows("residual", residual, x.dtype)
+        if out is None:
+            out = torch.empty(shape, dtype=x.dtype, device=self.device)
+        else:
+            self._check("out", out, x.dtype, tuple(shape))
+        o = self._rows("out", out, x.dtype)
+        N.check(
+            N.lib().hrs_linear(self._ctx, _TYPES[x.dtype], x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), self._vector("bias", bias, n),
+                               r.data_ptr() if r is not None else None, r.stride(0) if r is not None else 0, N.ACTIVATIONS[activation],
+                               o.data_ptr(), o.stride(0), m, n, k, self._queue()),
+            "hrs_linear",
+        )
+        return out
+
+    def layer_norm(self, x, weight, bias=None, eps=1e-12, residual=None, out=None):
+        """LayerNorm of x + residual over the last dimension (hrs_layer_norm): bf16, fp16 or fp32, weight and bias fp32
+        [N], statistics in fp32, one rounding.  Rows may lie at any stride; out may be x or residual."""
+        if x.dtype not in _TYPES:
+            raise ValueError(f"x must be bfloat16, float16 or float32, not {x.dtype}")
+        x2 = self._rows("x", x, x.dtype)
+        m, n = x2.shape
+        r = None
+        if residual is not None:
+            self._check("residual", residual, x.dtype, tuple(x.shape))
+            r = self._rows("residual", residual, x.dtype)
+        if out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=self.device)
+        else:
+            self._check("out", out, x.dtype, tuple(x.shape))
+        o = self._rows("out", out, x.dtype)
+        N.check(
+            N.lib().hrs_layer_norm(self._ctx, _TYPES[x.dtype], x2.data_ptr(), x2.stride(0), r.data_ptr() if r is not None else None, r.stride(0) if r is not None else 0,
+                                   self._vector("weight", weight, n), self._vector("bias", bias, n), float(eps), o.data_ptr(), o.stride(0), m, n, self._queue()),
+            "hrs_layer_norm",
+        )
+        return out
+
+    def _ints(self, name, t, n):
+        if t is None:
+            return None
+        self._check(name, t, torch.int32, (n,))
+        if n > 1 and t.stride(0) != 1:
+            raise ValueError(f"{name} must be contiguous")
+        return t.data_ptr()
+
+    def attention(self, q, k, v, q_offs=None, k_offs=None, q_lens=None, k_lens=None, prefix_lens=None, causal=False, scale=None, softcap=0.0,
+                  slopes=None, bias_table=None, max_q=None, max_k=None, out=None):
+        """Attention over packed or padded documents (hrs_attention), bf16 or fp16.
+
+        Packed: q [T, Hq, D], k and v [Tk, Hkv, D] with q_offs int32 [B + 1] (document b is the rows q_offs[b] .. q_offs[b + 1]),
+        k_offs likewise (q_offs where not given).  Padded: q [B, Sq, Hq, D], k and v [B, Sk, Hkv, D], with the number of
+        valid tokens of every document in q_lens / k_lens (int32 [B]; all where not given); queries behind q_lens give
+        zeros.  Query head h reads key head h // (Hq // Hkv).  The last query of a document stands at its last key; `causal` hides the
+        keys behind a query, except the first prefix_lens[b] (int32 [B]).  Scores are scale q . k (scale D ** -0.5 where
+        not given), capped to softcap tanh(. / softcap), with a bias by distance: -slopes[h] |j - p|, or
+        bias_table[h, clamp(j - p, -R, R) + R] (fp32 [Hq, 2 R + 1]).  A query that sees no key gives zeros.
+        max_q and max_k (longest documents of a packed batch) only shape the launch.  -> as q, contiguous."""
+        if q.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"q must be bfloat16 or float16, not {q.dtype}")
+        packed = q_offs is not None
+        nd = 3 if packed else 4
+        for name, t in (("q", q), ("k", k), ("v", v)):
+            self._check(name, t, q.dtype)
+            if t.dim() != nd:
+                raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {'[tokens, heads, dim] (packed)' if packed else '[documents, tokens, heads, dim]'}")
+            if t.stride(-1) != 1 and t.shape[-1] > 1:
+                raise ValueError(f"{name}: the elements of a head must be next to each other (last stride {t.stride(-1)})")
+        if k.shape != v.shape or k.shape[-1] != q.shape[-1] or (not packed and k.shape[0] != q.shape[0]):
+            raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit each other or q {tuple(q.shape)}")
+        if packed:
+            batch = q_offs.numel() - 1
+            if k_offs is None:
+                k_offs = q_offs
+                if k.shape[0] != q.shape[0]:
+                    raise ValueError(f"{k.shape[0]} key tokens for {q.shape[0]} query tokens: k_offs is needed")
+        else:
+            batch = q.shape[0]
+            if k_offs is not None:
+                raise ValueError("k_offs needs q_offs (packed documents)")
+        a = N.AttentionArgsC()
+        a.dtype, a.batch, a.q_heads, a.kv_heads, a.head_dim = _TYPES[q.dtype], batch, q.shape[-2], k.shape[-2], q.shape[-1]
+        a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+        a.q_stride[:], a.k_stride[:], a.v_stride[:] = (((0,) + t.stride()[:2] if packed else t.stride()[:3]) for t in (q, k, v))
+        a.q_rows, a.k_rows = q.shape[-3], k.shape[-3]
+        a.q_offs, a.k_offs = self._ints("q_offs", q_offs, batch + 1), self._ints("k_offs", k_offs, batch + 1)
+        a.q_lens, a.k_lens, a.prefix_lens = self._ints("q_lens", q_lens, batch), self._ints("k_lens", k_lens, batch), self._ints("prefix_lens", prefix_lens, batch)
+        a.causal, a.softcap = int(bool(causal)), float(softcap)
+        a.scale = float(scale) if scale is not None else q.shape[-1] ** -0.5 if q.shape[-1] else 1.0
+        a.slopes = self._vector("slopes", slopes, q.shape[-2])
+        if bias_table is not None:
+            if bias_table.dim() != 2 or bias_table.shape[0] != q.shape[-2] or bias_table.shape[1] % 2 == 0 or not bias_table.is_contiguous():
+                raise ValueError(f"bias_table: shape {tuple(bias_table.shape)}, expected contiguous [{q.shape[-2]}, 2 R + 1]")
+            self._check("bias_table", bias_table, torch.float32)
+            a.bias_table, a.bias_reach = bias_table.data_ptr(), bias_table.shape[1] // 2
+        a.max_q, a.max_k = max_q or 0, max_k or 0
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+        else:
+            self._check("out", out, q.dtype, tuple(q.shape))
+            if not out.is_contiguous():
+                raise ValueError("out must be contiguous")
+        a.out = out.data_ptr()
+        L = N.lib()
+        need = C.c_size_t()
+        N.check(L.hrs_attention_workspace(self._ctx, C.byref(a), C.byref(need)), "hrs_attention_workspace")
+        if need.value:
+            # from torch's allocator, on the current stream: two calls, or two captured graphs, never share it
+            workspace = torch.empty(need.value, dtype=torch.uint8, device=self.device)
+            a.workspace, a.workspace_bytes = workspace.data_ptr(), need.value
+        N.check(L.hrs_attention(self._ctx, C.byref(a), self._queue()), "hrs_attention")
+        return out
 
     # ---- synthetic inputs ----------------------------------------------------------------------
     def synth_rows(self, seed, row0, nrows, dim, normalize=True, out=None):

@@ -208,6 +208,65 @@ int hrs_encoder_release(hrs_ctx* ctx, hrs_encoder* enc);
 int hrs_encode(hrs_ctx* ctx, hrs_encoder* enc, const int32_t* ids_dev, const int32_t* lens_dev, int B, int S,
                float* out_dev, void* stream);
 
+/* ---- operators of an encoder layer --------------------------------------------------------- */
+/* What the forward pass behind SentenceTransformerEmbeddingFunction (scripts/chromadb_helper.py:58-71) is made of, for
+ * encoders of any width, with the score and mask forms that sentence encoders use.  Each call is one operator on device
+ * tensors of the caller; strides count elements.  No device memory is allocated, so the calls may be captured into a
+ * graph.  The calling thread's current device is left as it was. */
+enum hrs_type { HRS_TYPE_BF16 = 0, HRS_TYPE_FP16 = 1, HRS_TYPE_FP32 = 2 };
+enum hrs_activation { HRS_ACT_NONE = 0, HRS_ACT_RELU = 1, HRS_ACT_GELU = 2 /* erf */, HRS_ACT_GELU_TANH = 3, HRS_ACT_SILU = 4, HRS_ACT_TANH = 5 };
+
+/* y = act(x W^T + b) + r: x [M, K], W [N, K], r (nullable) and y [M, N] of type dtype (bf16 or fp16), rows ld* elements
+ * apart, elements of a row next to each other; bias (nullable) fp32 [N].  Sums, bias, activation and residual in fp32,
+ * one rounding at the end.  Any sizes, strides and alignments; rows of 16-byte aligned operands with strides and K that
+ * are multiples of 8 take the fastest kernels.  y may be r (element by element), not x or W.  K = 0 gives act(b) + r. */
+int hrs_linear(hrs_ctx* ctx, int dtype, const void* x_dev, int64_t ldx, const void* w_dev, int64_t ldw,
+               const float* bias_dev, const void* resid_dev, int64_t ldr, int act, void* y_dev, int64_t ldy, int64_t M,
+               int64_t N, int64_t K, void* stream);
+
+/* o_i = sum_j softmax_j(f(scale q_i . k_j) + bias(j - p_i)) v_j for every query i of every document and head.
+ * Query i of a document with lq queries and lk keys stands at p_i = i + lk - lq (the last query at the last key). */
+typedef struct hrs_attention_args {
+    const void *q, *k, *v;      /* [.., token, head, head_dim] of type dtype; elements of a head next to each other */
+    void* out;                  /* as q, contiguous: [documents, q_rows, q_heads, head_dim] or [q_rows, q_heads, head_dim] */
+    int dtype;                  /* HRS_TYPE_BF16 or HRS_TYPE_FP16 */
+    int batch;                  /* documents */
+    int q_heads, kv_heads;      /* query head h reads key head h / (q_heads / kv_heads) */
+    int head_dim;               /* a multiple of 8, at most 256 */
+    int causal;                 /* != 0: query i sees keys j <= p_i, and keys j < prefix_lens[document] */
+    float scale;                /* > 0 */
+    float softcap;              /* f(s) = softcap tanh(s / softcap); 0: f(s) = s */
+    int bias_reach;             /* see bias_table */
+    int64_t q_stride[3], k_stride[3], v_stride[3]; /* document (without offsets), token, head */
+    int64_t q_rows, k_rows;     /* tokens of a document, or of all documents where offsets are given */
+    /* documents packed back to back: document b has tokens offs[b] .. offs[b + 1]; int32 [batch + 1].  Rows behind the
+     * last document are left as they are.  Offsets and lengths are cut to the tensors they point into. */
+    const int32_t *q_offs, *k_offs;
+    /* valid tokens of document b, int32 [batch], nullable.  Queries behind q_lens[b] get zeros (not with q_offs);
+     * keys behind k_lens[b] are never read. */
+    const int32_t *q_lens, *k_lens;
+    const int32_t* prefix_lens; /* int32 [batch], nullable; with causal */
+    const float* slopes;        /* fp32 [q_heads], nullable: bias(d) = -slope |d| */
+    const float* bias_table;    /* fp32 [q_heads, 2 bias_reach + 1], nullable: bias(d) = table[h][clamp(d) + bias_reach] */
+    /* hints, 0 = unknown: longest lq and lk.  They shape the launch; results do not depend on their being right. */
+    int64_t max_q, max_k;
+    void* workspace;            /* hrs_attention_workspace bytes, 16-byte aligned; the call's own until it has run */
+    size_t workspace_bytes;
+} hrs_attention_args;
+/* A query that sees no key gets zeros.  Weights are rounded to dtype before they meet v; sums and statistics are fp32.
+ * k and v must be finite inside a document where a query of the same 128 rows may not see them (0 * inf is NaN). */
+int hrs_attention(hrs_ctx* ctx, const hrs_attention_args* args, void* stream);
+/* Bytes of workspace hrs_attention needs for these arguments (0 for most); the pointers in args are not looked at beyond
+ * being null or not. */
+int hrs_attention_workspace(hrs_ctx* ctx, const hrs_attention_args* args, size_t* bytes);
+
+/* y = (z - mean z) / sqrt(var z + eps) * gamma + beta with z = x + r, row by row: x, r (nullable) and y [M, N] of type
+ * dtype (bf16, fp16 or fp32), rows ld* elements apart; gamma and beta (nullable) fp32 [N].  z, mean and variance in
+ * fp32, one rounding at the end.  y may be x or r. */
+int hrs_layer_norm(hrs_ctx* ctx, int dtype, const void* x_dev, int64_t ldx, const void* resid_dev, int64_t ldr,
+                   const float* gamma_dev, const float* beta_dev, float eps, void* y_dev, int64_t ldy, int64_t M,
+                   int64_t N, void* stream);
+
 /* ---- the `where` filter -------------------------------------------------------------------- */
 /* Builds the row mask that hrs_score_topk takes from per-key value codes kept on the device, for the equality
  * forms of ChromaDB's `where` (scripts/chromadb_helper.py:265-266: {"system": S}; also $eq/$ne/$in/$nin/$and/$or).

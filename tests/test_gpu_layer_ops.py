@@ -1,0 +1,416 @@
+"""hrs_linear, hrs_attention and hrs_layer_norm against their definitions in 64 bits (oracle/layer_oracle.py), at the
+sizes, strides and masks where kernels like these go wrong; tolerances are the bounds derived there."""
+import itertools
+import random
+
+import pytest
+import torch
+
+from oracle import layer_oracle as LO
+
+pytestmark = pytest.mark.gpu
+TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+@pytest.fixture(scope="module")
+def eng():
+    from hybrid_rag_system_amd.engine import Engine
+
+    e = Engine(0)
+    yield e
+    e.close()
+
+
+def _gen(seed):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    return lambda *shape: torch.randn(shape, generator=g)
+
+
+def _close(got, want, bound, what=""):
+    got = got.cpu().double()
+    assert got.shape == want.shape
+    assert torch.isfinite(got).all(), what
+    over = (got - want).abs() / bound
+    at = over.argmax()
+    assert over.max() <= 1, (what, float(over.max()), int(at), float(got.flatten()[at]), float(want.flatten()[at]))
+
+
+# ---- linear ------------------------------------------------------------------------------------------
+SHAPES = [(1, 1, 1), (1, 384, 384), (3, 5, 7), (12, 1536, 384), (16, 17, 40), (17, 65, 33), (33, 40, 2048), (64, 64, 64), (63, 130, 96), (65, 129, 72), (100, 1024, 1000),
+          (129, 256, 64), (257, 1536, 384), (300, 520, 264), (512, 768, 128), (1000, 1024, 1024), (2100, 2056, 192), (4097, 256, 520)]
+
+
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_linear_matches_definition(eng, m, n, k, t):
+    dtype = TYPES[t]
+    rnd = _gen(m * 7 + n * 3 + k)
+    x, w, b, r = rnd(m, k).to(dtype), (rnd(n, k) * k**-0.5).to(dtype), rnd(n) * 0.3, rnd(m, n).to(dtype)
+    dx, dw, db, dr = x.cuda(), w.cuda(), b.cuda(), r.cuda()
+    acts = ["none", "relu", "gelu", "gelu_tanh", "silu", "tanh"]
+    for i, act in enumerate(acts if m * n < 300_000 else acts[(m + n) % 6 :: 3]):
+        use_b, use_r = (i + k) % 3 != 0, (i + m) % 2 == 0
+        want, bound = LO.linear(x, w, b if use_b else None, act, r if use_r else None, dtype)
+        got = eng.linear(dx, dw, db if use_b else None, activation=act, residual=dr if use_r else None)
+        _close(got, want, bound, (act, use_b, use_r))
+
+
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+@pytest.mark.parametrize("m,n,k,off,pad", [(20, 48, 64, 8, 8), (20, 48, 64, 1, 3), (150, 200, 136, 8, 16), (150, 200, 136, 3, 5), (150, 200, 136, 0, 1), (600, 320, 256, 8, 8), (600, 320, 256, 5, 0), (1, 320, 256, 5, 0)])
+def test_linear_on_slices(eng, m, n, k, off, pad, t):
+    """Operands that are windows of larger tensors (offset `off` and `pad` extra elements per row), the output one too:
+    what surrounds them holds NaN, and the output's surroundings stay as they were."""
+    dtype = TYPES[t]
+    rnd = _gen(off * 100 + pad)
+
+    def window(rows, cols):
+        whole = torch.full((rows + 2, off + cols + pad), float("nan"), dtype=dtype)
+        whole[1 : rows + 1, off : off + cols] = rnd(rows, cols).to(dtype)
+        dev = whole.cuda()
+        return whole[1 : rows + 1, off : off + cols], dev[1 : rows + 1, off : off + cols], dev
+
+    x, dx, _ = window(m, k)
+    w, dw, _ = window(n, k)
+    r, dr, _ = window(m, n)
+    _, dy, whole = window(m, n)
+    before = whole.clone()
+    b = rnd(n)
+    want, bound = LO.linear(x, w, b, "silu", r, dtype)
+    got = eng.linear(dx, dw, b.cuda(), activation="silu", residual=dr, out=dy)
+    assert got is dy
+    _close(got, want, bound)
+    inside = torch.zeros(whole.shape, dtype=torch.bool, device="cuda")
+    inside[1 : m + 1, off : off + n] = True
+    assert torch.equal(whole.view(torch.int16)[~inside], before.view(torch.int16)[~inside])
+    # in place over the residual, batched leading dimensions, a row repeated without memory (stride 0)
+    eng.linear(dx, dw, b.cuda(), activation="silu", residual=dr, out=dr)
+    assert torch.equal(dr, dy)
+    xb = x[:1].contiguous().cuda().expand(m, k)
+    want, bound = LO.linear(x[:1].expand(m, k), w, None, "none", None, dtype)
+    _close(eng.linear(xb, dw), want, bound)
+    if m % 10 == 0:
+        x3 = dx.contiguous().view(10, m // 10, k)
+        assert torch.equal(eng.linear(x3, dw).view(m, n), eng.linear(dx.contiguous(), dw))
+
+
+def test_linear_empty_and_infinite(eng):
+    x, w = torch.ones(4, 8, device="cuda", dtype=torch.bfloat16), torch.ones(6, 8, device="cuda", dtype=torch.bfloat16)
+    assert eng.linear(x[:0], w).shape == (0, 6) and eng.linear(x, w[:0]).shape == (4, 0)
+    b = torch.arange(6.0, device="cuda")
+    assert torch.equal(eng.linear(x[:, :0], w[:, :0], b, activation="relu").float(), b.expand(4, 6))
+    # an infinity or NaN in one row of x stays in that row; one in a row of W in that column
+    for rows in (4, 70, 700):
+        x = torch.randn(rows, 72, device="cuda").bfloat16()
+        w = torch.randn(200, 72, device="cuda").bfloat16()
+        clean = eng.linear(x, w)
+        x2, w2 = x.clone(), w.clone()
+        x2[2, 71], x2[3, 0] = float("nan"), float("inf")
+        w2[199, 5] = float("nan")
+        got = eng.linear(x2, w2)
+        keep = torch.ones(rows, 200, dtype=torch.bool, device="cuda")
+        keep[2:4], keep[:, 199] = False, False
+        assert torch.equal(got[keep], clean[keep])
+        assert torch.isnan(got[2]).all() and torch.isnan(got[:, 199]).all() and not torch.isfinite(got[3]).any()
+
+
+# ---- layer norm --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("t", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("m,n", [(1, 1), (1, 384), (3, 7), (5, 8), (12, 384), (4, 511), (9, 512), (7, 513), (130, 1024), (6, 1025), (33, 2048), (3, 2051), (5, 4096), (2, 4099), (3, 8192), (2, 8200), (2, 20001)])
+def test_layer_norm_matches_definition(eng, m, n, t):
+    dtype = TYPES[t]
+    rnd = _gen(m * 11 + n)
+    x, r, g, b = (rnd(m, n) * 2 + 0.5).to(dtype), rnd(m, n).to(dtype), 1 + 0.2 * rnd(n), 0.3 * rnd(n)
+    for use_r, use_b, eps in ((True, True, 1e-12), (False, True, 1e-5), (True, False, 1e-12)):
+        want, bound = LO.layer_norm(x, g, b if use_b else None, eps, r if use_r else None, dtype)
+        got = eng.layer_norm(x.cuda(), g.cuda(), b.cuda() if use_b else None, eps=eps, residual=r.cuda() if use_r else None)
+        _close(got, want, bound, (use_r, use_b))
+
+
+@pytest.mark.parametrize("n", [384, 385, 2500, 9000])
+def test_layer_norm_rows_with_a_large_mean_and_strides(eng, n):
+    """A mean a thousand times the deviation (a difference of sums of squares would lose the variance), windows of larger
+    tensors, in place."""
+    rnd = _gen(n)
+    whole = (rnd(6, n + 9) + 1000).float()
+    x, g, b = whole[1:5, 3 : 3 + n], 1 + 0.1 * rnd(n), 0.1 * rnd(n)
+    want, bound = LO.layer_norm(x, g, b, dtype=torch.float32)
+    dev = whole.cuda()
+    dx = dev[1:5, 3 : 3 + n]
+    got = eng.layer_norm(dx, g.cuda(), b.cuda())
+    _close(got, want, bound)
+    eng.layer_norm(dx, g.cuda(), b.cuda(), out=dx)
+    assert torch.equal(dx, got)
+    inside = torch.zeros(whole.shape, dtype=torch.bool)
+    inside[1:5, 3 : 3 + n] = True
+    assert torch.equal(dev.cpu()[~inside], whole[~inside])
+    # a constant row is beta
+    assert torch.equal(eng.layer_norm(torch.full((2, n), 3.0, device="cuda"), g.cuda(), b.cuda()).cpu(), b.expand(2, n))
+    assert eng.layer_norm(dx[:0], g.cuda()).shape == (0, n)
+
+
+# ---- attention ---------------------------------------------------------------------------------------
+def _attention_case(eng, layout, qlens, klens, heads, kv_heads, dim, t, causal=False, prefix=None, cap=0.0, bias=None, reach=0, scale=None, seed=0, size=1.0, sq=None, sk=None, strided=False,
+                    max_q=None, max_k=None):
+    """Builds one call, runs it, checks every document; what stands behind documents is NaN."""
+    dtype = TYPES[t]
+    rnd = _gen(seed + 17)
+    nan = float("nan")
+
+    def make(layout, lens, width, h, f=1.0):
+        if layout == "packed":
+            total = sum(lens)
+            body = (rnd(total, h, dim) * f).to(dtype)
+            host = torch.cat([body, torch.full((5, h, dim), nan, dtype=dtype)])  # rows behind the last document
+        else:
+            host = torch.full((len(lens), width, h, dim), nan, dtype=dtype)
+            for b, n in enumerate(lens):
+                host[b, :n] = (rnd(n, h, dim) * f).to(dtype)
+        return host
+
+    sq, sk = sq or max(qlens), sk or max(klens)
+    q, k, v = make(layout, qlens, sq, heads, size), make(layout, klens, sk, kv_heads, size), make(layout, klens, sk, kv_heads)
+    if layout != "packed":
+        q = torch.nan_to_num(q)
+    dq, dk, dv = q.cuda(), k.cuda(), v.cuda()
+    if strided:  # one tensor [.., q heads + 2 kv heads, dim + 8], as a fused projection leaves it
+        def place(parts):
+            whole = torch.full(parts[0].shape[:-2] + (sum(p.shape[-2] for p in parts), dim + 8), nan, dtype=dtype, device="cuda")
+            views, at = [], 0
+            for p in parts:
+                view = whole[..., at : at + p.shape[-2], :dim]
+                view.copy_(p)
+                views.append(view)
+                at += p.shape[-2]
+            return views
+        if q.shape[:-2] == k.shape[:-2]:
+            dq, dk, dv = place([dq, dk, dv])
+        else:
+            (dq,), (dk, dv) = place([dq]), place([dk, dv])
+    slopes = torch.tensor([2.0 ** (-8.0 * (i + 1) / heads) for i in range(heads)]) if bias == "slope" else None
+    table = rnd(heads, 2 * reach + 1) if bias == "table" else None
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    kw = dict(causal=causal, softcap=cap, scale=scale, slopes=slopes.cuda() if bias == "slope" else None, bias_table=table.cuda() if bias == "table" else None,
+              prefix_lens=ints(prefix) if prefix else None, max_q=max_q, max_k=max_k)
+    if layout == "packed":
+        offs = lambda lens: ints(list(itertools.accumulate([0] + list(lens))))
+        out = torch.full(q.shape, 7.0, dtype=dtype, device="cuda")
+        got = eng.attention(dq, dk, dv, q_offs=offs(qlens), k_offs=offs(klens), out=out, **kw)
+        assert got is out and (got[sum(qlens):] == 7).all()  # rows behind the last document stay
+    else:
+        got = eng.attention(dq, dk, dv, q_lens=ints(qlens) if any(n != sq for n in qlens) else None, k_lens=ints(klens), **kw)
+    assert got.is_contiguous()
+    at_q = at_k = 0
+    for b, (lq, lk) in enumerate(zip(qlens, klens)):
+        qb = q[at_q : at_q + lq] if layout == "packed" else q[b]
+        kb, vb = (k[at_k : at_k + lk], v[at_k : at_k + lk]) if layout == "packed" else (k[b], v[b])
+        gb = got[at_q : at_q + lq] if layout == "packed" else got[b]
+        at_q, at_k = at_q + lq, at_k + lk
+        want, bound = LO.attention(qb, kb, vb, lq, lk, causal, prefix[b] if prefix else None, scale, cap, slopes, table, dtype)
+        if want.numel():
+            _close(gb, want, bound + 1e-30, ("document", b, lq, lk))
+    return got
+
+
+@pytest.mark.parametrize("dim", [8, 32, 40, 64, 80, 128, 136, 256])
+@pytest.mark.parametrize("layout", ["packed", "padded"])
+def test_attention_of_ragged_documents(eng, layout, dim):
+    lens = [1, 31, 32, 33, 64, 65, 127, 128, 129, 200, 2]
+    t = "bf16" if dim % 16 == 0 else "fp16"
+    _attention_case(eng, layout, lens, lens, 3, 3, dim, t, seed=dim)
+    _attention_case(eng, layout, lens, lens, 4, 2, dim, t, causal=True, cap=20.0, bias="slope", size=3.0, seed=dim + 1)
+    _attention_case(eng, layout, lens, lens, 2, 1, dim, t, bias="table", reach=9, seed=dim + 2, strided=True)
+
+
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+@pytest.mark.parametrize("bias,reach", [(None, 0), ("slope", 0), ("table", 0), ("table", 1), ("table", 70)])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("causal,prefix", [(False, None), (True, None), (True, [5, 0, 1000, 64, 3])])
+def test_attention_forms(eng, t, bias, reach, cap, causal, prefix):
+    """Every bias with every cap and mask; documents whose queries and keys differ in number both ways (with causal order
+    the first queries of the third document then see nothing, and the last document has no key at all)."""
+    _attention_case(eng, "packed", [7, 100, 90, 130, 5], [7, 160, 40, 130, 0], 4, 2, 64, t, causal, prefix, cap, bias, reach, size=2.0, seed=reach)
+    _attention_case(eng, "padded", [70, 33, 64, 0, 70], [70, 150, 20, 9, 0], 2, 2, 32, t, causal, prefix, cap, bias, reach, size=2.0, seed=reach + 1, sk=160)
+
+
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 8, 64), (8, 2, 128), (16, 1, 64), (6, 2, 80), (4, 4, 256), (71, 1, 32)])
+@pytest.mark.parametrize("queries", [1, 2, 9])
+def test_attention_of_few_queries_over_many_keys(eng, t, heads, kv_heads, dim, queries):
+    """Serving: the newest tokens of every document over all its keys, from one key to thousands."""
+    klens = [4000, 1, 63, 64, 65, 1025, queries, 300]
+    for cap, bias, reach in ((0.0, None, 0), (25.0, "slope", 0), (0.0, "table", 33)):
+        _attention_case(eng, "padded", [queries] * 8, klens, heads, kv_heads, dim, t, True, None, cap, bias, reach, seed=queries, sk=4100)
+    _attention_case(eng, "padded", [queries], [9001], heads, kv_heads, dim, t, True, [4500], 0.0, "slope", seed=queries + 1)
+    _attention_case(eng, "packed", [queries] * 8, klens, heads, kv_heads, dim, t, True, seed=queries + 2, max_q=queries, max_k=4000)
+
+
+@pytest.mark.parametrize("max_q,max_k", [(None, None), (1, 1), (16, 4000), (100000, 100000)])
+def test_attention_hints_only_shape_the_launch(eng, max_q, max_k):
+    lens = [300, 1, 0, 77, 513, 64]
+    _attention_case(eng, "packed", lens, lens, 2, 2, 64, "bf16", True, None, 0.0, "slope", max_q=max_q, max_k=max_k, seed=3)
+
+
+def test_attention_of_long_documents(eng):
+    _attention_case(eng, "packed", [1500, 700], [1500, 700], 2, 1, 64, "bf16", bias="slope", seed=1)
+    _attention_case(eng, "padded", [1111], [2222], 1, 1, 128, "fp16", True, [1700], 40.0, "table", 100, seed=2, size=3.0)
+
+
+def test_attention_scores_far_apart(eng):
+    """Scores in the thousands, a scale of its own, weights that are one-hot: the running maximum has to move."""
+    _attention_case(eng, "padded", [90], [900], 2, 2, 64, "bf16", size=9.0, scale=1.0, seed=5)
+    _attention_case(eng, "padded", [1], [3000], 4, 1, 128, "bf16", size=7.0, scale=2.0, seed=6)
+
+
+def test_attention_table_of_infinities(eng):
+    """-inf in the table hides a distance (a row of nothing else is zero), the type's lowest value does not: alone in a
+    row it is a uniform weight."""
+    q, k, v = (torch.randn(1, 70, 1, 64, device="cuda").bfloat16() for _ in range(3))
+    low = torch.finfo(torch.float32).min
+    out = eng.attention(q, k, v, bias_table=torch.full((1, 1), float("-inf"), device="cuda"))
+    assert (out == 0).all()
+    out = eng.attention(q, k, v, bias_table=torch.full((1, 1), low, device="cuda"))
+    want = v.double().mean(1, keepdim=True).expand(-1, 70, -1, -1)
+    assert ((out.double() - want).abs() <= 2.0**-8 * want.abs() + 2.0**-8 * v.double().abs().mean(1, keepdim=True)).all()
+    table = torch.tensor([[float("-inf"), 0.0, low]], device="cuda")  # own position only; keys behind at the lowest value
+    out = eng.attention(q, k, v, bias_table=table)
+    assert torch.equal(out, v)
+
+
+def test_attention_bad_offsets_stay_inside(eng):
+    """Offsets and lengths that point outside are cut to the tensors (documented); nothing outside out is written."""
+    q = torch.randn(100, 2, 64, device="cuda").bfloat16()
+    room = torch.full((300, 2, 64), 7.0, device="cuda").bfloat16()
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    out = eng.attention(q, q, q, q_offs=ints(-50, 40, 2**31 - 1), out=room[100:200])
+    assert (room[:100] == 7).all() and (room[200:] == 7).all()
+    assert torch.equal(out, eng.attention(q, q, q, q_offs=ints(0, 40, 100)))
+    assert torch.equal(eng.attention(q, q, q, q_offs=ints(0, 100), k_lens=ints(2**31 - 1), causal=True, prefix_lens=ints(-7)), eng.attention(q, q, q, q_offs=ints(0, 100), causal=True))
+    # offsets that step back make an empty document
+    assert torch.equal(eng.attention(q, q, q, q_offs=ints(0, 60, 20, 20), out=room[100:200])[:60], eng.attention(q[:60], q[:60], q[:60], q_offs=ints(0, 60))[:60])
+
+
+def test_attention_nan_in_one_query_stays_there(eng):
+    q, k, v = (torch.randn(2, 200, 2, 64, device="cuda").bfloat16() for _ in range(3))
+    clean = eng.attention(q, k, v)
+    q2 = q.clone()
+    q2[0, 5, 1, 3] = float("nan")
+    got = eng.attention(q2, k, v)
+    assert torch.isnan(got[0, 5, 1]).all()
+    got[0, 5, 1] = clean[0, 5, 1]
+    assert torch.equal(got, clean)
+
+
+def test_random_cases(eng):
+    rng = random.Random(11)
+    for i in range(40):
+        layout = rng.choice(["packed", "padded"])
+        nb = rng.randint(1, 6)
+        qlens = [rng.choice([0, 1, rng.randint(1, 40), rng.randint(1, 300)]) for _ in range(nb)]
+        qlens[0] = max(qlens[0], 1)
+        klens = [rng.choice([n, rng.randint(0, 400)]) for n in qlens]
+        klens[0] = max(klens[0], 1)
+        kv = rng.choice([1, 2, 3])
+        causal = rng.random() < 0.6
+        prefix = [rng.randint(0, 300) for _ in range(nb)] if causal and rng.random() < 0.4 else None
+        bias = rng.choice([None, "slope", "table"])
+        _attention_case(eng, layout, qlens, klens, kv * rng.choice([1, 2, 5]), kv, rng.choice([8, 16, 32, 48, 64, 96, 128, 192]), rng.choice(["bf16", "fp16"]), causal, prefix,
+                        rng.choice([0.0, 15.0]), bias, rng.randint(0, 90), seed=i, strided=rng.random() < 0.4, size=rng.choice([1.0, 3.0]))
+
+
+# ---- streams, graphs, a run of them together -----------------------------------------------------------
+def test_captured_and_replayed(eng):
+    """The three operators captured into two graphs, replayed alternately with eager work in between: every replay gives
+    the eager results."""
+    def layer(x, offs, w, wo, g):
+        t = x.shape[0]
+        qkv = eng.linear(x, w).view(t, 3, 2, 64)
+        ctx = eng.attention(qkv[:, 0], qkv[:, 1], qkv[:, 2], q_offs=offs, causal=True, max_q=int(t))
+        return eng.layer_norm(eng.linear(ctx.view(t, 128), wo, activation="gelu", residual=x), g)
+
+    sets = []
+    for t, n in ((300, 3), (1, 1)):
+        x = torch.randn(t, 128, device="cuda").bfloat16()
+        offs = torch.linspace(0, t, n + 1, device="cuda").int()
+        w, wo, g = (torch.randn(384, 128, device="cuda") * 0.1).bfloat16(), (torch.randn(128, 128, device="cuda") * 0.1).bfloat16(), torch.ones(128, device="cuda")
+        layer(x, offs, w, wo, g)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = layer(x, offs, w, wo, g)
+        sets.append((x, offs, w, wo, g, graph, y))
+    for i in range(4):
+        for x, offs, w, wo, g, graph, y in sets:
+            x.copy_(torch.randn_like(x))
+            graph.replay()
+            want = layer(x, offs, w, wo, g)
+            torch.cuda.synchronize()
+            assert torch.equal(y, want), i
+
+
+def test_on_another_stream(eng):
+    x, w = torch.randn(500, 256, device="cuda").bfloat16(), torch.randn(256, 256, device="cuda").bfloat16()
+    want = eng.linear(x, w)
+    q = torch.randn(4, 1, 8, 64, device="cuda").bfloat16()
+    k = torch.randn(4, 5000, 2, 64, device="cuda").bfloat16()
+    want_a = eng.attention(q, k, k)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        y, a = eng.linear(x, w), eng.attention(q, k, k)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(y, want) and torch.equal(a, want_a)
+    for _ in range(3):  # the same bits every time
+        assert torch.equal(eng.linear(x, w), want) and torch.equal(eng.attention(q, k, k), want_a)
+
+
+def test_refusals(eng):
+    bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device="cuda")
+    f32 = lambda *s: torch.zeros(*s, device="cuda")
+    from hybrid_rag_system_amd._native import HrsError
+
+    for bad in (
+        lambda: eng.linear(f32(2, 8), f32(4, 8)),
+        lambda: eng.linear(bf(2, 8), bf(4, 8).half()),
+        lambda: eng.linear(bf(2, 8), bf(4, 9)),
+        lambda: eng.linear(bf(2, 8), bf(4, 8), bias=bf(4)),
+        lambda: eng.linear(bf(2, 8), bf(4, 8), bias=f32(5)),
+        lambda: eng.linear(bf(2, 8), bf(4, 8), bias=f32(8)[::2]),
+        lambda: eng.linear(bf(2, 8), bf(4, 8), activation="swish"),
+        lambda: eng.linear(bf(2, 8), bf(4, 8), residual=bf(2, 5)),
+        lambda: eng.linear(bf(2, 8), bf(4, 8), out=bf(3, 4)),
+        lambda: eng.linear(bf(2, 16)[:, ::2], bf(4, 8)),
+        lambda: eng.linear(bf(4, 6, 8)[:, :3], bf(4, 8)),
+        lambda: eng.linear(bf(2, 8).cpu(), bf(4, 8)),
+        lambda: eng.layer_norm(bf(2, 8), bf(8)),
+        lambda: eng.layer_norm(bf(2, 8), f32(9)),
+        lambda: eng.layer_norm(bf(2, 8).double(), f32(8)),
+        lambda: eng.layer_norm(bf(2, 8), f32(8), residual=bf(1, 8)),
+        lambda: eng.attention(bf(1, 4, 2, 64), bf(1, 4, 2, 64), bf(1, 4, 2, 32)),
+        lambda: eng.attention(bf(4, 2, 64), bf(4, 2, 64), bf(4, 2, 64)),
+        lambda: eng.attention(bf(1, 4, 2, 64), bf(1, 4, 2, 64), bf(1, 4, 2, 64), k_lens=torch.zeros(1, device="cuda", dtype=torch.int64)),
+        lambda: eng.attention(bf(1, 4, 2, 64), bf(1, 4, 2, 64), bf(1, 4, 2, 64), k_offs=torch.zeros(2, device="cuda", dtype=torch.int32)),
+        lambda: eng.attention(bf(4, 2, 64), bf(5, 2, 64), bf(5, 2, 64), q_offs=torch.zeros(2, device="cuda", dtype=torch.int32)),
+        lambda: eng.attention(bf(1, 4, 2, 64), bf(1, 4, 2, 64), bf(1, 4, 2, 64), bias_table=f32(2, 4)),
+        lambda: eng.attention(bf(1, 4, 2, 64), bf(1, 4, 2, 64), bf(1, 4, 2, 64), slopes=f32(3)),
+    ):
+        with pytest.raises(ValueError):
+            bad()
+    for bad, word in (
+        (lambda: eng.attention(bf(1, 4, 3, 64), bf(1, 4, 2, 64), bf(1, 4, 2, 64)), "multiple"),
+        (lambda: eng.attention(bf(1, 4, 2, 60), bf(1, 4, 2, 60), bf(1, 4, 2, 60)), "head_dim"),
+        (lambda: eng.attention(bf(1, 4, 2, 264), bf(1, 4, 2, 264), bf(1, 4, 2, 264)), "head_dim"),
+        (lambda: eng.attention(bf(1, 4, 2, 64), bf(1, 4, 2, 64), bf(1, 4, 2, 64), scale=0.0), "scale"),
+        (lambda: eng.attention(bf(1, 4, 2, 64), bf(1, 4, 2, 64), bf(1, 4, 2, 64), softcap=-1.0), "softcap"),
+        (lambda: eng.attention(bf(1, 4, 2, 64), bf(1, 4, 2, 64), bf(1, 4, 2, 64), slopes=f32(2), bias_table=f32(2, 3)), "exclude"),
+        (lambda: eng.attention(bf(1, 4, 2, 64), bf(1, 4, 2, 64), bf(1, 4, 2, 64), prefix_lens=torch.zeros(1, device="cuda", dtype=torch.int32)), "causal"),
+        (lambda: eng.layer_norm(bf(2, 8), f32(8), eps=-1.0), "eps"),
+    ):
+        with pytest.raises(HrsError, match=word):
+            bad()
+    x = bf(8, 8)
+    with pytest.raises(HrsError, match="may not be x"):
+        eng.linear(x, bf(8, 8), out=x)
+    q = bf(1, 4, 2, 64)
+    with pytest.raises(HrsError, match="may not be an input"):
+        eng.attention(q, bf(1, 4, 2, 64), bf(1, 4, 2, 64), out=q)
