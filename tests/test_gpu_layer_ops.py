@@ -94,6 +94,19 @@ def test_linear_on_slices(eng, m, n, k, off, pad, t):
         assert torch.equal(eng.linear(x3, dw).view(m, n), eng.linear(dx.contiguous(), dw))
 
 
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+@pytest.mark.parametrize("m,n,k", [(4097, 2050, 200), (2049, 4104, 64), (2600, 3592, 328), (5000, 2000, 8), (8192, 2048, 128), (9000, 2304, 72)])
+def test_linear_large(eng, m, n, k, t):
+    """Sizes that take the largest tiles, several of them per workgroup: a depth of one stage and of a part of one, edges
+    on every side."""
+    dtype = TYPES[t]
+    rnd = _gen(m + n + k)
+    x, w, b, r = rnd(m, k).to(dtype), (rnd(n, k) * k**-0.5).to(dtype), rnd(n), rnd(m, n).to(dtype)
+    for act, use_r in (("gelu", False), ("none", True)):
+        want, bound = LO.linear(x, w, b, act, r if use_r else None, dtype)
+        _close(eng.linear(x.cuda(), w.cuda(), b.cuda(), activation=act, residual=r.cuda() if use_r else None), want, bound, act)
+
+
 def test_linear_empty_and_infinite(eng):
     x, w = torch.ones(4, 8, device="cuda", dtype=torch.bfloat16), torch.ones(6, 8, device="cuda", dtype=torch.bfloat16)
     assert eng.linear(x[:0], w).shape == (0, 6) and eng.linear(x, w[:0]).shape == (4, 0)
