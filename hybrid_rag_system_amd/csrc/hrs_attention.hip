@@ -24,8 +24,13 @@ struct AttnArgs {
     int64_t q_rows, k_rows;  // tokens per document, or of all documents where offsets are given
     int batch, heads, kv_heads, group, dim, tiles;
     int causal, reach;
-    float scale2;             // scale log2 e
-    float cap2, cap_in;       // cap log2 e; 2 log2 e scale / cap
+    float scale2;        // scale log2 e
+    float cap2, cap_in;  // cap log2 e; 2 log2 e scale / cap
+    // long documents: `chunk` keys per workgroup, unnormalised sums [chunks][rows][dim] and (m, l) [chunks][rows]
+    int chunk, chunks;
+    int64_t part_rows;
+    float* part;
+    float2* part_ml;
 };
 
 enum { BIAS_NONE = 0, BIAS_SLOPE = 1, BIAS_TABLE = 2 };
@@ -93,8 +98,10 @@ __device__ __forceinline__ float score2(const AttnArgs& a, float s, float slope2
     return x;
 }
 
+// ---- any alignment, any table ------------------------------------------------------------------------
+// 128 rows per workgroup, 32 per wave; pieces of K and V pass through registers one by one.
 template <typename T, int DP, int BIAS, bool CAP>
-__global__ __launch_bounds__(256) void k_attend(AttnArgs a) {
+__global__ __launch_bounds__(256) void k_attend_any(AttnArgs a) {
     typedef typename vec_of<T>::x8 x8;
     constexpr int KT = DP <= 128 ? 64 : 32, PPR = DP / 8, NB = KT / 32, ND = DP / 32, NS = DP / 16;
     __shared__ __attribute__((aligned(16))) char kl[KT * DP * 2];
@@ -223,28 +230,574 @@ __global__ __launch_bounds__(256) void k_attend(AttnArgs a) {
     }
 }
 
+// ---- aligned operands: K and V by LDS-DMA --------------------------------------------------------------
+template <int DP>
+__device__ __forceinline__ int swizzle_k(int i) { return DP == 32 ? (i >> 1) & 3 : i & 7; }
+template <int DP>
+__device__ __forceinline__ int swizzle_v(int i) { return DP == 32 ? i & 2 : (i & 3) << 1; }
+
+// A row of the tile and what it is allowed to see.
+struct RowPlace {
+    int64_t row;  // row / group: token, row % group: head of this key head's group
+    bool live;
+    int token, head, pos, lim;
+};
+__device__ __forceinline__ int limit_of(const AttnArgs& a, const DocRange& d, int pos, int prefix) {
+    if (!a.causal) return d.lk;
+    const int lim = pos + 1 > prefix ? pos + 1 : prefix;
+    return lim < 0 ? 0 : lim > d.lk ? d.lk : lim;
+}
+__device__ __forceinline__ RowPlace row_place(const AttnArgs& a, const DocRange& d, int hk, int prefix, int64_t row) {
+    RowPlace r;
+    r.row = row;
+    r.live = row < (int64_t)d.lq * a.group;
+    r.token = (int)(row / a.group);
+    r.head = hk * a.group + (int)(row % a.group);
+    r.pos = r.token + d.lk - d.lq;
+    r.lim = r.live ? limit_of(a, d, r.pos, prefix) : 0;
+    return r;
+}
+
+// The state of one lane's row (query c = lane % 32 of the wave; the wave's halves hold different keys and dimensions).
+template <typename T, int DP, int NB, int BIAS, bool CAP, bool FIXED>
+struct Attend {
+    typedef typename vec_of<T>::x8 x8;
+    static constexpr int ND = DP / 32, NS = DP / 16, KT = NB * 32;
+    // With a slope the bias of a tile wholly before (or behind) all positions of the wave is linear in j: its part that
+    // varies over the tile enters as the initial value of the products, so it costs no instruction.
+    static constexpr bool RAMP = BIAS == BIAS_SLOPE && !CAP && DP <= 64;
+    x8 qf[NS];
+    f32x16 acc[ND];
+    f32x16 up[RAMP ? NB : 1], down[RAMP ? NB : 1];
+    float m, l, slope2, edge_lo, edge_hi;
+    int pos, lim;
+    int pos_min, pos_max, lim_min, lim_max;  // over the wave's live rows
+    int table_at;                            // of the row's head in the LDS copy, at distance 0
+    bool tame;                               // biases are of a size that scores do not vanish beside
+
+    __device__ __forceinline__ void open(const AttnArgs& a, const DocRange& d, int b, int hk, int prefix, int64_t row0, const RowPlace& r, const float* table) {
+        const int lane = threadIdx.x & 63, h = lane >> 5;
+        const T* qp = (const T*)a.q + b * a.q_sb + (d.q0 + r.token) * a.q_st + r.head * a.q_sh + h * 8;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) qf[s] = (r.live && s * 16 + h * 8 < a.dim) ? *(const x8*)(qp + s * 16) : (x8)((T)0.f);
+        const int64_t rows = (int64_t)d.lq * a.group, last = row0 + 31 < rows - 1 ? row0 + 31 : rows - 1;
+        pos_min = (int)(row0 / a.group) + d.lk - d.lq;
+        pos_max = (int)(last / a.group) + d.lk - d.lq;
+        const bool any = row0 < rows;
+        lim_min = any ? limit_of(a, d, pos_min, prefix) : 0;
+        lim_max = any ? limit_of(a, d, pos_max, prefix) : 0;
+        pos_min = __builtin_amdgcn_readfirstlane(pos_min);
+        pos_max = __builtin_amdgcn_readfirstlane(pos_max);
+        lim_min = __builtin_amdgcn_readfirstlane(lim_min);
+        lim_max = __builtin_amdgcn_readfirstlane(lim_max);
+        pos = r.live ? r.pos : pos_max;  // (rows behind the last one are computed along, inside the table, and dropped)
+        lim = r.lim;
+        m = FIXED ? 0.f : -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int i = 0; i < ND; ++i) acc[i] = (f32x16)(0.f);
+        if constexpr (BIAS == BIAS_SLOPE) slope2 = r.live ? a.slopes[r.head] * LOG2E : 0.f;
+        if constexpr (RAMP) {
+            const float per = slope2 / a.scale2;
+            tame = !__any(!(fabsf(per) < 1e15f));
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    up[n][e] = per * (float)(n * 32 + 8 * (e >> 2) + (e & 3));
+                    down[n][e] = -up[n][e];
+                }
+        }
+        if constexpr (BIAS == BIAS_TABLE) {
+            table_at = (r.head - hk * a.group) * (2 * a.reach + 1) + a.reach;
+            edge_lo = table[table_at - a.reach];
+            edge_hi = table[table_at + a.reach];
+            tame = !__any(!(fabsf(edge_lo) < 1e30f && fabsf(edge_hi) < 1e30f));
+        }
+    }
+
+    // The row's sum over both halves of the wave; a row that is none has nothing.
+    __device__ __forceinline__ void close(bool live) {
+        l += swap_halves(l);
+        if (!live) {
+            l = 0.f;
+            m = FIXED ? 0.f : -INFINITY;
+#pragma unroll
+            for (int i = 0; i < ND; ++i) acc[i] = (f32x16)(0.f);
+        }
+    }
+
+    // Keys j0 .. j0 + KT - 1, of which those below lim are seen; kl, vl: their tile in LDS.
+    __device__ __forceinline__ void tile(const AttnArgs& a, const char* kl, const char* vl, const float* table, int j0) {
+        const int lane = threadIdx.x & 63, h = lane >> 5, c32 = lane & 31;
+        const bool before = tame && j0 + KT - 1 <= pos_min, behind = tame && j0 >= pos_max;  // (of a slope)
+        f32x16 s[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            const int i = n * 32 + c32;
+            if constexpr (RAMP) {
+                if (before)
+                    s[n] = mfma32(*(const x8*)(kl + i * (DP * 2) + ((h ^ swizzle_k<DP>(i)) << 4)), qf[0], up[n]);
+                else if (behind)
+                    s[n] = mfma32(*(const x8*)(kl + i * (DP * 2) + ((h ^ swizzle_k<DP>(i)) << 4)), qf[0], down[n]);
+                else
+                    s[n] = mfma32(*(const x8*)(kl + i * (DP * 2) + ((h ^ swizzle_k<DP>(i)) << 4)), qf[0], (f32x16)(0.f));
+            } else {
+                s[n] = mfma32(*(const x8*)(kl + i * (DP * 2) + ((h ^ swizzle_k<DP>(i)) << 4)), qf[0], (f32x16)(0.f));
+            }
+#pragma unroll
+            for (int t = 1; t < NS; ++t) s[n] = mfma32(*(const x8*)(kl + i * (DP * 2) + (((2 * t + h) ^ swizzle_k<DP>(i)) << 4)), qf[t], s[n]);
+        }
+        if constexpr (RAMP) {
+            // The scores are read behind a branch here, and the compiler has left a read too close behind the last product
+            // on such a path (three of the eleven wait states that the result of a 32 x 32 product needs).
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("s_nop 11");
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // x = s mul + add is the score in base 2
+        float mul = CAP ? 1.f : a.scale2, add = 0.f;
+        const int d0 = j0 + 4 * h - pos;  // distance of this lane's first key
+        if constexpr (CAP) {
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[n][e] = fmaf(-2.f * a.cap2, rcp_hw(1.f + exp2_hw(s[n][e] * a.cap_in)), a.cap2);
+        }
+        if constexpr (BIAS == BIAS_SLOPE) {
+            if (RAMP && before) {
+                add = slope2 * (float)d0;
+            } else if (RAMP && behind) {
+                add = -slope2 * (float)d0;
+            } else {
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[n][e] = fmaf(-slope2, fabsf((float)(d0 + n * 32 + 8 * (e >> 2) + (e & 3))), CAP ? s[n][e] : s[n][e] * a.scale2);
+                mul = 1.f;
+            }
+        }
+        if constexpr (BIAS == BIAS_TABLE) {
+            if (tame && j0 + KT - 1 <= pos_min - a.reach) {
+                add = edge_lo;
+            } else if (tame && j0 >= pos_max + a.reach) {
+                add = edge_hi;
+            } else {
+                const bool inner = j0 + KT - 1 - pos_min <= a.reach && j0 - pos_max >= -a.reach;
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        int d = d0 + n * 32 + 8 * (e >> 2) + (e & 3);
+                        if (!inner) d = d < -a.reach ? -a.reach : d > a.reach ? a.reach : d;
+                        s[n][e] = (CAP ? s[n][e] : s[n][e] * a.scale2) + table[table_at + d];
+                    }
+                mul = 1.f;
+            }
+        }
+        if (j0 + KT > lim_min) {  // (else every row of the wave sees the whole tile)
+            const int left = lim - (j0 + 4 * h);
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[n][e] = n * 32 + 8 * (e >> 2) + (e & 3) < left ? s[n][e] : -INFINITY;
+        }
+        if constexpr (!FIXED) {
+            float top = s[0][0];
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = fmaxf(top, s[n][e]);
+            top = fmaf(top, mul, add);
+            top = fmaxf(top, swap_halves(top));
+            if (__any(top > m)) {  // (in a long row the maximum rarely moves after the first tiles)
+                const float m_new = fmaxf(m, top);
+                const float keep = exp2_hw(m - (m_new == -INFINITY ? 0.f : m_new));
+                m = m_new;
+                l *= keep;
+#pragma unroll
+                for (int i = 0; i < ND; ++i) acc[i] *= keep;
+            }
+            add -= m == -INFINITY ? 0.f : m;  // nothing seen so far: every weight is exp2(-inf) = 0
+        }
+        x8 pf[2 * NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float w = FIXED ? exp2_hw(s[n][e]) : exp2_hw(fmaf(s[n][e], mul, add));
+                l += w;
+                pf[2 * n + (e >> 3)][e & 7] = (T)w;
+            }
+#pragma unroll
+        for (int t = 0; t < 2 * NB; ++t)
+#pragma unroll
+            for (int i = 0; i < ND; ++i) {
+                union {
+                    s16x4 half[2];
+                    x8 all;
+                } vf;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int key = t * 16 + e * 8 + 4 * h + ((lane & 15) >> 2), col = i * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+                    vf.half[e] = lds_read_tr(vl + key * (DP * 2) + (((col >> 3) ^ swizzle_v<DP>(key)) << 4) + (col & 7) * 2);
+                }
+                acc[i] = mfma32(vf.all, pf[t], acc[i]);
+            }
+    }
+};
+
+// The wave's share of the DMA of one tile: KT rows of K and of V, NI instructions of 1 KB each.
+template <int DP, int KT, int NWAVES>
+struct TileLoad {
+    static constexpr int PPR = DP / 8, RPI = 64 / PPR, NI = KT / RPI / NWAVES;
+    int kof[NI], vof[NI], kp[NI], vp[NI], row[NI];
+    __device__ __forceinline__ void open(const AttnArgs& a, int wave) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+            row[j] = (wave * NI + j) * RPI + lane / PPR;
+            const int pk = (lane % PPR) ^ swizzle_k<DP>(row[j]), pv = (lane % PPR) ^ swizzle_v<DP>(row[j]);
+            // (a piece behind the head's dimension repeats the first: it meets zeros of q, or ends in columns not stored)
+            kp[j] = pk * 8 < a.dim ? pk * 16 : 0;
+            vp[j] = pv * 8 < a.dim ? pv * 16 : 0;
+            kof[j] = row[j] * (int)(a.k_st * 2) + kp[j];
+            vof[j] = row[j] * (int)(a.v_st * 2) + vp[j];
+        }
+    }
+    // Rows j0 .. of K and V to LDS; rows behind the last key repeat it, so what stands there is never read.
+    template <typename T>
+    __device__ __forceinline__ void issue(const AttnArgs& a, const T* k, const T* v, int j0, int lk, uint32_t kl, uint32_t vl, int wave) {
+        const char* kb = uniform_ptr(k + j0 * a.k_st);
+        const char* vb = uniform_ptr(v + j0 * a.v_st);
+        const bool whole = j0 + KT <= lk;
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+            const int use = lk - 1 - j0;
+            glds16_asm(kb, whole ? kof[j] : (row[j] < use ? row[j] : use) * (int)(a.k_st * 2) + kp[j], kl + (wave * NI + j) * 1024);
+        }
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+            const int use = lk - 1 - j0;
+            glds16_asm(vb, whole ? vof[j] : (row[j] < use ? row[j] : use) * (int)(a.v_st * 2) + vp[j], vl + (wave * NI + j) * 1024);
+        }
+    }
+};
+
+// Table rows of a key head's group, in base 2 (a finite entry stays finite, also the type's lowest value).
+__device__ __forceinline__ void stage_table(const AttnArgs& a, int hk, float* dst) {
+    const int n = a.group * (2 * a.reach + 1);
+    const float* src = a.table + (int64_t)hk * n;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) dst[i] = fmaxf(src[i] * LOG2E, fminf(src[i], -1e30f));
+}
+
+__device__ __forceinline__ int64_t out_row(const AttnArgs& a, const DocRange& d, int b, int token, int head) {
+    return ((a.q_offs ? 0 : b * a.q_rows) + d.q0 + token) * a.heads + head;
+}
+
+// One lane's row of O^T: registers 4 g .. 4 g + 3 are dimensions 8 g + 4 h .. + 3 of 32.  One exchange between the wave's
+// halves per two pieces gives either half whole 16-byte pieces.
+template <typename T, int ND>
+__device__ __forceinline__ void store_row(const AttnArgs& a, const f32x16 (&acc)[ND], float inv, int64_t orow, bool write) {
+    const int h = (threadIdx.x >> 5) & 1;
+    T* op = (T*)a.out + orow * a.dim;
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; g += 2) {
+            union {
+                T v[4];
+                u32x2 u;
+            } lo, hi;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                lo.v[e] = (T)(acc[i][4 * g + e] * inv);
+                hi.v[e] = (T)(acc[i][4 * g + 4 + e] * inv);
+            }
+            const auto r0 = __builtin_amdgcn_permlane32_swap(lo.u.x, hi.u.x, false, false);
+            const auto r1 = __builtin_amdgcn_permlane32_swap(lo.u.y, hi.u.y, false, false);
+            u32x4 o;
+            o.x = r0[0];
+            o.y = r1[0];
+            o.z = r0[1];
+            o.w = r1[1];
+            const int d = i * 32 + (g + h) * 8;
+            if (write && d < a.dim) __builtin_memcpy(op + d, &o, 16);
+        }
+}
+template <int ND>
+__device__ __forceinline__ void store_part(const AttnArgs& a, const f32x16 (&acc)[ND], float m, float l, int chunk, int64_t orow, bool write) {
+    const int h = (threadIdx.x >> 5) & 1;
+    const int64_t at = chunk * a.part_rows + orow;
+    if (!write) return;
+    float* op = a.part + at * a.dim;
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int d = i * 32 + g * 8 + h * 4;
+            const f32x4 o = {acc[i][4 * g], acc[i][4 * g + 1], acc[i][4 * g + 2], acc[i][4 * g + 3]};
+            if (d < a.dim) *(f32x4*)(op + d) = o;
+        }
+    if (h == 0) a.part_ml[at] = make_float2(m, l);
+}
+// 1 / l; a row that sees nothing is zero, NaN stays NaN.
+__device__ __forceinline__ float inverse(float l) { return l > 0.f || l != l ? 1.f / l : 0.f; }
+
+// ---- many rows: 128 per workgroup, 32 per wave ---------------------------------------------------------
+// All four waves read the tiles of 64 keys (32 for heads wider than 128) that they fetch together, two buffers deep.
+template <typename T, int DP, int BIAS, bool CAP, bool FIXED>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attend_rows(AttnArgs a) {
+    constexpr int NB = DP <= 128 ? 2 : 1, KT = NB * 32, TILE = KT * DP * 2;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const float* table = (const float*)(lds + 4 * TILE);
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int id = spread_over_xcds((int)blockIdx.x, (int)gridDim.x);
+    const int chunk = id % a.chunks;
+    id /= a.chunks;
+    const int t0 = a.tiles - 1 - id % a.tiles;  // causal: the longest rows first
+    id /= a.tiles;
+    const int hk = id % a.kv_heads, b = id / a.kv_heads;
+    const DocRange dr = doc_range(a, b);
+    const int64_t rows = (int64_t)dr.lq * a.group, rows_all = (int64_t)dr.q_total * a.group;
+    const T* kbase = (const T*)a.k + b * a.k_sb + dr.k0 * a.k_st + hk * a.k_sh;
+    const T* vbase = (const T*)a.v + b * a.v_sb + dr.k0 * a.v_st + hk * a.v_sh;
+    const int prefix = a.prefix ? a.prefix[b] : 0;
+    const int from = chunk * a.chunk;
+    if (from > 0 && from >= dr.lk) return;
+    if constexpr (BIAS == BIAS_TABLE) {
+        stage_table(a, hk, (float*)(lds + 4 * TILE));
+        __syncthreads();
+    }
+    TileLoad<DP, KT, 4> load;
+    load.open(a, wv);
+    const uint32_t l0 = lds_addr_of(lds);
+
+    for (int64_t row0 = (int64_t)t0 * 128; row0 < rows_all; row0 += (int64_t)a.tiles * 128) {
+        const RowPlace r = row_place(a, dr, hk, prefix, row0 + wv * 32 + (lane & 31));
+        Attend<T, DP, NB, BIAS, CAP, FIXED> st;
+        st.open(a, dr, b, hk, prefix, row0 + wv * 32, r, table);
+        // keys that any row of the workgroup sees
+        int need = 0;
+        if (row0 < rows) {
+            const int64_t last = row0 + 127 < rows - 1 ? row0 + 127 : rows - 1;
+            need = limit_of(a, dr, (int)(last / a.group) + dr.lk - dr.lq, prefix);
+            if (need > from + a.chunk) need = from + a.chunk;
+        }
+        int buf = 0;
+        if (from < need) load.issue(a, kbase, vbase, from, dr.lk, l0, l0 + TILE, wv);
+        for (int j0 = from; j0 < need; j0 += KT, buf ^= 1) {
+            wait_all_barrier();  // the tile has landed; everyone has read the one before
+            if (j0 + KT < need) load.issue(a, kbase, vbase, j0 + KT, dr.lk, l0 + (buf ^ 1) * 2 * TILE, l0 + (buf ^ 1) * 2 * TILE + TILE, wv);
+            if (j0 < st.lim_max) st.tile(a, lds + buf * 2 * TILE, lds + buf * 2 * TILE + TILE, table, j0);
+        }
+        st.close(r.live);
+        const bool write = r.row < rows_all;
+        const int64_t orow = out_row(a, dr, b, r.token, r.head);
+        if (a.chunks == 1)
+            store_row<T>(a, st.acc, inverse(st.l), orow, write);
+        else
+            store_part(a, st.acc, st.m, st.l, chunk, orow, write);
+        if (row0 + (int64_t)a.tiles * 128 < rows_all) __syncthreads();  // (the next rows fetch over the last tile)
+    }
+}
+
+// ---- few rows: up to 32 per document and key head --------------------------------------------------------
+// The waves of a workgroup share the keys instead of the rows: wave w takes tiles w, w + NW, .. of 32 keys through an LDS
+// ring of its own, without a barrier, and the waves' sums meet at the end in a fixed order.
+template <typename T, int DP, int NW, int BIAS, bool CAP, bool FIXED>
+__global__ __launch_bounds__(64 * NW) void k_attend_few(AttnArgs a) {
+    constexpr int KT = 32, TILE = KT * DP * 2, ND = DP / 32, RING = 4 * TILE;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const float* table = (const float*)(lds + NW * RING);
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int id = spread_over_xcds((int)blockIdx.x, (int)gridDim.x);
+    const int hk = id % a.kv_heads;
+    id /= a.kv_heads;
+    const int chunk = id % a.chunks, b = id / a.chunks;
+    const DocRange dr = doc_range(a, b);
+    const int64_t rows_all = (int64_t)dr.q_total * a.group;
+    const T* kbase = (const T*)a.k + b * a.k_sb + dr.k0 * a.k_st + hk * a.k_sh;
+    const T* vbase = (const T*)a.v + b * a.v_sb + dr.k0 * a.v_st + hk * a.v_sh;
+    const int prefix = a.prefix ? a.prefix[b] : 0;
+    const int from = chunk * a.chunk;
+    if (from > 0 && from >= dr.lk) return;
+    if constexpr (BIAS == BIAS_TABLE) {
+        stage_table(a, hk, (float*)(lds + NW * RING));
+        __syncthreads();
+    }
+    TileLoad<DP, KT, 1> load;
+    load.open(a, 0);
+    char* mine = lds + wv * RING;
+    const uint32_t l0 = lds_addr_of(lds) + wv * RING;
+
+    for (int64_t row0 = 0; row0 < rows_all; row0 += 32) {
+        const RowPlace r = row_place(a, dr, hk, prefix, row0 + (lane & 31));
+        Attend<T, DP, 1, BIAS, CAP, FIXED> st;
+        st.open(a, dr, b, hk, prefix, row0, r, table);
+        int need = st.lim_max;
+        if (need > from + a.chunk) need = from + a.chunk;
+        int buf = 0;
+        const int first = from + wv * KT;
+        if (first < need) load.issue(a, kbase, vbase, first, dr.lk, l0, l0 + TILE, 0);
+        for (int j0 = first; j0 < need; j0 += NW * KT, buf ^= 1) {
+            // this wave's reads of the other buffer are done (the products that needed them are under way)
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (j0 + NW * KT < need) {
+                load.issue(a, kbase, vbase, j0 + NW * KT, dr.lk, l0 + (buf ^ 1) * 2 * TILE, l0 + (buf ^ 1) * 2 * TILE + TILE, 0);
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * TileLoad<DP, KT, 1>::NI) : "memory");
+            } else {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
+            st.tile(a, mine + buf * 2 * TILE, mine + buf * 2 * TILE + TILE, table, j0);
+        }
+        st.close(r.live);
+        // join: wave 0 takes the others' (m, l, O) in order
+        __syncthreads();
+        float* sum = (float*)lds;  // [NW - 1][ND * 16 + 2][64]
+        constexpr int EACH = (ND * 16 + 2) * 64;
+        static_assert((NW - 1) * EACH * 4 <= NW * RING, "the sums fit where the tiles were");
+        if (wv > 0) {
+            float* to = sum + (wv - 1) * EACH + lane;
+            to[0] = st.m;
+            to[64] = st.l;
+#pragma unroll
+            for (int i = 0; i < ND; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) to[(2 + i * 16 + e) * 64] = st.acc[i][e];
+        }
+        __syncthreads();
+        if (wv == 0) {
+#pragma unroll 1
+            for (int w = 0; w < NW - 1; ++w) {
+                const float* of = sum + w * EACH + lane;
+                const float m2 = of[0], l2 = of[64], top = fmaxf(st.m, m2), base = top == -INFINITY ? 0.f : top;
+                const float f1 = FIXED ? 1.f : exp2_hw(st.m - base), f2 = FIXED ? 1.f : exp2_hw(m2 - base);
+                st.m = top;
+                st.l = st.l * f1 + l2 * f2;
+#pragma unroll
+                for (int i = 0; i < ND; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) st.acc[i][e] = st.acc[i][e] * f1 + of[(2 + i * 16 + e) * 64] * f2;
+            }
+            const bool write = r.row < rows_all;
+            const int64_t orow = out_row(a, dr, b, r.token, r.head);
+            if (a.chunks == 1)
+                store_row<T>(a, st.acc, inverse(st.l), orow, write);
+            else
+                store_part(a, st.acc, st.m, st.l, chunk, orow, write);
+        }
+        if (row0 + 32 < rows_all) __syncthreads();
+    }
+}
+
+// ---- the chunks of a row joined --------------------------------------------------------------------------
+// One wave per row: o = sum_c o_c 2^(m_c - m) / sum_c l_c 2^(m_c - m), chunks in order.
+template <typename T>
+__global__ __launch_bounds__(256) void k_attend_join(AttnArgs a, int rows_hint) {
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const int groups = (rows_hint + 3) / 4;
+    const int b = blockIdx.x / groups;
+    const DocRange dr = doc_range(a, b);
+    const int64_t rows_all = (int64_t)dr.q_total * a.heads;
+    const int n = dr.lk <= a.chunk ? 1 : (dr.lk + a.chunk - 1) / a.chunk;
+    for (int64_t row = (int64_t)(blockIdx.x % groups) * 4 + wv; row < rows_all; row += (int64_t)groups * 4) {
+        const int64_t at = ((a.q_offs ? 0 : b * a.q_rows) + dr.q0) * a.heads + row;
+        float m = -INFINITY;
+        for (int c = 0; c < n; ++c) m = fmaxf(m, a.part_ml[c * a.part_rows + at].x);
+        const float base = m == -INFINITY ? 0.f : m;
+        float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+        const int d = lane * 4;
+        for (int c = 0; c < n; ++c) {
+            const float2 ml = a.part_ml[c * a.part_rows + at];
+            const float f = exp2_hw(ml.x - base);
+            l += ml.y * f;
+            if (d < a.dim) {
+                const f32x4 v = *(const f32x4*)(a.part + (c * a.part_rows + at) * a.dim + d);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] += v[e] * f;
+            }
+        }
+        const float inv = inverse(l);
+        if (d < a.dim) {
+            T* op = (T*)a.out + at * a.dim + d;
+            T v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (T)(o[e] * inv);
+            __builtin_memcpy(op, v, 8);
+        }
+    }
+}
+
 // ---- host side ---------------------------------------------------------------------------------------
-template <typename T, int DP, int BIAS, bool CAP>
-static int launch_attend(const AttnArgs& a, hipStream_t st) {
-    const int64_t grid = (int64_t)a.batch * a.kv_heads * a.tiles;
+#define ATTN_TABLE_LDS 16384  // bytes of table rows that a workgroup keeps in LDS; larger ones are read from memory
+
+struct AttnPlan {
+    bool fast = false, few = false;
+    int64_t longest_q = 0, part_rows = 0;
+    size_t bytes = 0;  // of workspace
+};
+
+template <typename K>
+static int launch_attend(hrs_ctx* ctx, hrs_per_device_once& attr, K kernel, int threads, int lds, int64_t grid, const AttnArgs& a, hipStream_t st) {
     HRS_REQUIRE(grid < (1ll << 31), "hrs_attention: %lld workgroups", (long long)grid);
-    hipLaunchKernelGGL((k_attend<T, DP, BIAS, CAP>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    if (lds > 65536 && attr.need(ctx->device)) {
+        HRS_CHECK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        attr.done(ctx->device);
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(threads), lds, st, a);
     HRS_CHECK_HIP(hipGetLastError());
     return HRS_OK;
 }
+template <typename T, int DP, int BIAS, bool CAP, bool FIXED>
+static int launch_fast(hrs_ctx* ctx, const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
+    static hrs_per_device_once once_few, once_rows;
+    const int table = BIAS == BIAS_TABLE ? a.group * (2 * a.reach + 1) * 4 : 0;
+    const int64_t pairs = (int64_t)a.batch * a.kv_heads;
+    if (p.few) {
+        constexpr int NW = DP == 256 ? 2 : 4;
+        return launch_attend(ctx, once_few, k_attend_few<T, DP, NW, BIAS, CAP, FIXED>, 64 * NW, NW * 4 * 32 * DP * 2 + table, pairs * a.chunks, a, st);
+    }
+    constexpr int KT = DP <= 128 ? 64 : 32;
+    return launch_attend(ctx, once_rows, k_attend_rows<T, DP, BIAS, CAP, FIXED>, 256, 4 * KT * DP * 2 + table, pairs * a.tiles * a.chunks, a, st);
+}
+template <typename T, int DP, int BIAS, bool CAP>
+static int launch_form(hrs_ctx* ctx, const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
+    if (!p.fast) {
+        static hrs_per_device_once once;
+        return launch_attend(ctx, once, k_attend_any<T, DP, BIAS, CAP>, 256, 0, (int64_t)a.batch * a.kv_heads * a.tiles, a, st);
+    }
+    // Capped scores without a bias lie within +-cap: in bf16, whose range is that of fp32, the weights need no running
+    // maximum (2^+-80, their sum over 2^30 keys and its product with v stay inside fp32).
+    if constexpr (CAP && BIAS == BIAS_NONE && __is_same(T, __bf16)) {
+        if (a.cap2 <= 80.f) return launch_fast<T, DP, BIAS, CAP, true>(ctx, a, p, st);
+    }
+    return launch_fast<T, DP, BIAS, CAP, false>(ctx, a, p, st);
+}
 template <typename T, int DP>
-static int launch_attend_form(const AttnArgs& a, hipStream_t st) {
+static int launch_dim(hrs_ctx* ctx, const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
     const bool cap = a.cap2 > 0.f;
-    if (a.table) return cap ? launch_attend<T, DP, BIAS_TABLE, true>(a, st) : launch_attend<T, DP, BIAS_TABLE, false>(a, st);
-    if (a.slopes) return cap ? launch_attend<T, DP, BIAS_SLOPE, true>(a, st) : launch_attend<T, DP, BIAS_SLOPE, false>(a, st);
-    return cap ? launch_attend<T, DP, BIAS_NONE, true>(a, st) : launch_attend<T, DP, BIAS_NONE, false>(a, st);
+    if (a.table) return cap ? launch_form<T, DP, BIAS_TABLE, true>(ctx, a, p, st) : launch_form<T, DP, BIAS_TABLE, false>(ctx, a, p, st);
+    if (a.slopes) return cap ? launch_form<T, DP, BIAS_SLOPE, true>(ctx, a, p, st) : launch_form<T, DP, BIAS_SLOPE, false>(ctx, a, p, st);
+    return cap ? launch_form<T, DP, BIAS_NONE, true>(ctx, a, p, st) : launch_form<T, DP, BIAS_NONE, false>(ctx, a, p, st);
 }
 template <typename T>
-static int launch_attend_dim(const AttnArgs& a, hipStream_t st) {
-    if (a.dim <= 32) return launch_attend_form<T, 32>(a, st);
-    if (a.dim <= 64) return launch_attend_form<T, 64>(a, st);
-    if (a.dim <= 128) return launch_attend_form<T, 128>(a, st);
-    return launch_attend_form<T, 256>(a, st);
+static int launch_type(hrs_ctx* ctx, const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
+    int rc;
+    if (a.dim <= 32)
+        rc = launch_dim<T, 32>(ctx, a, p, st);
+    else if (a.dim <= 64)
+        rc = launch_dim<T, 64>(ctx, a, p, st);
+    else if (a.dim <= 128)
+        rc = launch_dim<T, 128>(ctx, a, p, st);
+    else
+        rc = launch_dim<T, 256>(ctx, a, p, st);
+    if (rc || a.chunks == 1) return rc;
+    const int64_t rows = p.longest_q * a.heads, groups = (rows + 3) / 4;
+    HRS_REQUIRE(rows < (1ll << 30) && groups * a.batch < (1ll << 31), "hrs_attention: %lld rows to join", (long long)rows);
+    hipLaunchKernelGGL(k_attend_join<T>, dim3((unsigned)(groups * a.batch)), dim3(256), 0, st, a, (int)rows);
+    HRS_CHECK_HIP(hipGetLastError());
+    return HRS_OK;
 }
 
 static int attention_args(const hrs_attention_args* p, AttnArgs& a) {
@@ -300,28 +853,90 @@ static int attention_args(const hrs_attention_args* p, AttnArgs& a) {
     return HRS_OK;
 }
 
-extern "C" int hrs_attention(hrs_ctx* ctx, const hrs_attention_args* p, void* stream) {
-    HRS_REQUIRE(ctx && p, "hrs_attention: null argument");
-    AttnArgs a;
+// How the work is cut, from the arguments alone (never from device data).
+static AttnPlan plan_attention(hrs_ctx* ctx, const hrs_attention_args* p, AttnArgs& a) {
+    AttnPlan plan;
+    // without a hint for packed documents: twice their mean
+    const int64_t mean_q = a.q_offs && a.batch ? (2 * a.q_rows + a.batch - 1) / a.batch : a.q_rows;
+    const int64_t mean_k = a.k_offs && a.batch ? (2 * a.k_rows + a.batch - 1) / a.batch : a.k_rows;
+    auto hint = [](int64_t given, int64_t otherwise, int64_t all) {
+        const int64_t v = given > 0 ? given : otherwise;
+        return v < 1 ? (int64_t)1 : v < all ? v : all;
+    };
+    plan.longest_q = hint(p->max_q, mean_q, a.q_rows);
+    const int64_t longest_k = hint(p->max_k, mean_k, a.k_rows), rows = plan.longest_q * a.group;
+    a.tiles = (int)((rows + 127) / 128);
+    a.chunks = 1;
+    a.chunk = 1 << 30;
+    // 16-byte pieces, and 64 rows of K or V within the 2^31 bytes that a DMA's lane offset spans
+    const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out;
+    const int64_t strides = a.q_sb | a.q_st | a.q_sh | a.k_sb | a.k_st | a.k_sh | a.v_sb | a.v_st | a.v_sh;
+    plan.fast = at % 16 == 0 && strides % 8 == 0 && a.k_st < (1 << 23) && a.v_st < (1 << 23) &&
+                (!a.table || (int64_t)a.group * (2 * a.reach + 1) * 4 <= ATTN_TABLE_LDS);
+    if (!plan.fast) return plan;
+    plan.few = rows <= 32;
+    // Too few workgroups for the card: long documents are cut into chunks of keys, joined by a second launch.
+    const int64_t groups = (int64_t)a.batch * a.kv_heads * (plan.few ? 1 : a.tiles), want = 4 * (int64_t)ctx->num_cu;
+    if (groups < want / 2 && longest_k > 1024) {
+        int64_t chunks = want / groups, most = longest_k / 512;
+        if (chunks > most) chunks = most;
+        if (chunks > 64) chunks = 64;
+        if (chunks > 1) {
+            a.chunk = (int)(((longest_k + chunks - 1) / chunks + 127) / 128 * 128);
+            // every key of every document has its chunk, whatever the hint said
+            a.chunks = (int)((a.k_rows + a.chunk - 1) / a.chunk);
+            if (a.chunks > 256) {  // (a hint far below the documents' room)
+                a.chunks = 256;
+                a.chunk = (int)((a.k_rows / 256 + 128) / 128 * 128);
+            }
+            a.chunks = (int)((a.k_rows + a.chunk - 1) / a.chunk);
+        }
+        if (a.chunks > 1) {
+            plan.part_rows = (a.q_offs ? a.q_rows : a.batch * a.q_rows) * a.heads;
+            plan.bytes = (size_t)a.chunks * plan.part_rows * (a.dim * sizeof(float) + sizeof(float2));
+        } else {
+            a.chunks = 1;
+            a.chunk = 1 << 30;
+        }
+    }
+    a.part_rows = plan.part_rows;
+    return plan;
+}
+
+static int check_attention(hrs_ctx* ctx, const hrs_attention_args* p, AttnArgs& a) {
     int rc = attention_args(p, a);
     if (rc) return rc;
     if (a.batch == 0 || a.q_rows == 0) return HRS_OK;
     HRS_REQUIRE(a.q && a.out && (a.k_rows == 0 || (a.k && a.v)), "hrs_attention: null operand");
     HRS_REQUIRE(a.out != a.q && a.out != a.k && a.out != a.v, "hrs_attention: out may not be an input");
     HRS_REQUIRE(((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out) % 2 == 0, "hrs_attention: an operand is not aligned to its elements");
-    hrs_device_scope dev(ctx->device);
-    HRS_CHECK_HIP(dev.err);
-    int64_t longest = p->max_q > 0 && p->max_q < a.q_rows ? p->max_q : a.q_rows;
-    if (a.q_offs && p->max_q <= 0) longest = (a.q_rows + a.batch - 1) / a.batch;  // without a hint: twice the mean
-    a.tiles = (int)((longest * a.group + 127) / 128);
-    return p->dtype == HRS_TYPE_BF16 ? launch_attend_dim<__bf16>(a, (hipStream_t)stream) : launch_attend_dim<_Float16>(a, (hipStream_t)stream);
+    (void)ctx;
+    return HRS_OK;
 }
 
 extern "C" int hrs_attention_workspace(hrs_ctx* ctx, const hrs_attention_args* p, size_t* bytes) {
     HRS_REQUIRE(ctx && p && bytes, "hrs_attention_workspace: null argument");
-    AttnArgs a;
-    int rc = attention_args(p, a);
-    if (rc) return rc;
     *bytes = 0;
+    AttnArgs a;
+    int rc = check_attention(ctx, p, a);
+    if (rc || a.batch == 0 || a.q_rows == 0) return rc;
+    *bytes = plan_attention(ctx, p, a).bytes;
     return HRS_OK;
+}
+
+extern "C" int hrs_attention(hrs_ctx* ctx, const hrs_attention_args* p, void* stream) {
+    HRS_REQUIRE(ctx && p, "hrs_attention: null argument");
+    AttnArgs a;
+    int rc = check_attention(ctx, p, a);
+    if (rc || a.batch == 0 || a.q_rows == 0) return rc;
+    const AttnPlan plan = plan_attention(ctx, p, a);
+    if (plan.bytes) {
+        HRS_REQUIRE(p->workspace && p->workspace_bytes >= plan.bytes && (uintptr_t)p->workspace % 16 == 0,
+                    "hrs_attention: a workspace of %zu bytes (given: %zu), 16-byte aligned, is needed", plan.bytes, p->workspace ? p->workspace_bytes : (size_t)0);
+        a.part = (float*)p->workspace;
+        a.part_ml = (float2*)(a.part + (size_t)a.chunks * plan.part_rows * a.dim);
+    }
+    hrs_device_scope dev(ctx->device);
+    HRS_CHECK_HIP(dev.err);
+    return p->dtype == HRS_TYPE_BF16 ? launch_type<__bf16>(ctx, a, plan, (hipStream_t)stream) : launch_type<_Float16>(ctx, a, plan, (hipStream_t)stream);
 }

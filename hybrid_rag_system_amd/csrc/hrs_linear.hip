@@ -83,10 +83,6 @@ struct TilePos {
 };
 // Workgroups go round the 8 XCDs, each with an L2 of its own: every XCD gets a consecutive run of tiles, and a run walks
 // `deep` tiles of tokens by all features at a time, so that the tiles in flight on an XCD share operand rows.
-__device__ __forceinline__ int spread_over_xcds(int block, int grid) {
-    const int x = block & 7, q = grid >> 3, r = grid & 7;
-    return x * q + (x < r ? x : r) + (block >> 3);
-}
 template <int BM, int BN>
 __device__ __forceinline__ TilePos tile_at(int id, int tm, int tn) {
     constexpr int deep = 8;

@@ -49,6 +49,12 @@ __device__ __forceinline__ typename vec_of<T>::x8 load8_any(const T* p, int n) {
     return v;
 }
 
+// Consecutive workgroups go round the 8 XCDs, each with an L2 of its own: renumbered so that an XCD has a consecutive run.
+__device__ __forceinline__ int spread_over_xcds(int block, int grid) {
+    const int x = block & 7, q = grid >> 3, r = grid & 7;
+    return x * q + (x < r ? x : r) + (block >> 3);
+}
+
 // ---- activations -----------------------------------------------------------------------------------
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_GELU_TANH = 3, ACT_SILU = 4, ACT_TANH = 5 };
 

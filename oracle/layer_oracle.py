@@ -110,6 +110,9 @@ def attention(q, k, v, lq, lk, causal=False, prefix=None, scale=None, cap=0.0, s
         x = s
         if slopes is not None:
             x = x - slopes[h].double() * dist.abs()
+            # a bias linear over a tile of 64 keys may enter the products as their initial value (up to 64 slope), which
+            # each of the dim / 16 + 1 accumulations then rounds beside, and leave with the tile's own offset
+            ds = ds + 2 * (dim / 16 + 3) * 64 * slopes[h].double().abs() * F
         if table is not None:
             reach = table.shape[1] // 2
             x = x + table[h].double()[dist.clamp(-reach, reach) + reach]
