@@ -5,6 +5,7 @@ no MI355X is present when a context is created, the call raises.
 """
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("HRS_LIBRARY") or os.path.join(_HERE, "libhrs.so")  # HRS_LIBRARY: another build of the same ABI (A/B timing)
@@ -80,6 +81,11 @@ class AttentionArgsC(C.Structure):
         + [(n, C.c_void_p) for n in ("q_offs", "k_offs", "q_lens", "k_lens", "prefix_lens", "slopes", "bias_table")]
         + [("max_q", C.c_int64), ("max_k", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
     )
+
+
+# hrs_attention_args as one pack() (field by field through ctypes a call would cost several us more)
+ATTENTION_ARGS = struct.Struct("@4P6i2fi9q2q7P2qPN")
+assert ATTENTION_ARGS.size == C.sizeof(AttentionArgsC)
 
 
 class HrsError(RuntimeError):

@@ -474,79 +474,83 @@ class Engine:
         except RuntimeError:
             raise ValueError(f"{name}: rows at strides {tuple(t.stride())} have no common stride") from None
 
-    def _vector(self, name, t, n):
+    def _matrix(self, name, t, dtype, n):
+        """_rows for what most calls pass: a matrix that is as it should be."""
+        if t.dtype is dtype and t.device == self.device and t.dim() == 2 and t.shape[1] == n and (t.stride(1) == 1 or n <= 1):
+            return t
+        return self._rows(name, t, dtype, n)
+
+    def _vector(self, name, t, n, dtype=torch.float32):
         if t is None:
             return None
-        self._check(name, t, torch.float32, (n,))
+        if t.dtype is not dtype or t.device != self.device or t.shape != (n,):
+            self._check(name, t, dtype, (n,))
         if n > 1 and t.stride(0) != 1:
             raise ValueError(f"{name} must be contiguous")
         return t.data_ptr()
 
+    def _result(self, out, shape, dtype):
+        if out is None:
+            return torch.empty(shape, dtype=dtype, device=self.device)
+        self._check("out", out, dtype, tuple(shape))
+        return out
+
     def _queue(self):
-        return torch.cuda.current_stream(self.device).cuda_stream
+        """The current stream of this engine's GPU (whatever the current GPU is)."""
+        return torch._C._cuda_getCurrentRawStream(self.device.index)  # (torch.cuda.current_stream() takes 2 us)
 
     def linear(self, x, weight, bias=None, activation="none", residual=None, out=None):
         """act(x @ weight.T + bias) + residual in one kernel (hrs_linear): x [.., K] and weight [N, K] bf16 or fp16, bias
         fp32 [N], residual [.., N] as x; activation "none", "relu", "gelu" (erf), "gelu_tanh", "silu" or "tanh".  Rows may
         lie at any stride.  Sums, bias, activation and residual in fp32, one rounding.  out (as the result) may be
         residual, not x or weight."""
-        if x.dtype not in (torch.bfloat16, torch.float16):
-            raise ValueError(f"x must be bfloat16 or float16, not {x.dtype}")
-        if activation not in N.ACTIVATIONS:
+        dtype = x.dtype
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"x must be bfloat16 or float16, not {dtype}")
+        act = N.ACTIVATIONS.get(activation)
+        if act is None:
             raise ValueError(f"unknown activation {activation!r}: one of {', '.join(N.ACTIVATIONS)}")
         if weight.dim() != 2:
             raise ValueError(f"weight: shape {tuple(weight.shape)}, expected [N, K]")
         n, k = weight.shape
-        x2, w = self._rows("x", x, x.dtype, k), self._rows("weight", weight, x.dtype)
-        shape = x.shape[:-1] + (n,)
+        x2, w = self._matrix("x", x, dtype, k), self._matrix("weight", weight, dtype, k)
         m = x2.shape[0]
-        r = None
+        shape = (m, n) if x.dim() == 2 else x.shape[:-1] + (n,)
+        r, ldr = None, 0
         if residual is not None:
-            self._check("residual", residual, x.dtype, tuple(shape))
-            r = self._rows("residual", residual, x.dtype)
-        if out is None:
-            out = torch.empty(shape, dtype=x.dtype, device=self.device)
-        else:
-            self._check("out", out, x.dtype, tuple(shape))
-        o = self._rows("out", out, x.dtype)
-        N.check(
-            N.lib().hrs_linear(self._ctx, _TYPES[x.dtype], x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), self._vector("bias", bias, n),
-                               r.data_ptr() if r is not None else None, r.stride(0) if r is not None else 0, N.ACTIVATIONS[activation],
-                               o.data_ptr(), o.stride(0), m, n, k, self._queue()),
-            "hrs_linear",
-        )
+            if residual.shape != shape:
+                self._check("residual", residual, dtype, tuple(shape))
+            r2 = self._matrix("residual", residual, dtype, n)
+            r, ldr = r2.data_ptr(), r2.stride(0)
+        out = self._result(out, shape, dtype)
+        o = self._matrix("out", out, dtype, n)
+        rc = N.lib().hrs_linear(self._ctx, _TYPES[dtype], x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), self._vector("bias", bias, n), r, ldr, act, o.data_ptr(), o.stride(0), m, n, k,
+                                self._queue())
+        N.check(rc, "hrs_linear")
         return out
 
     def layer_norm(self, x, weight, bias=None, eps=1e-12, residual=None, out=None):
         """LayerNorm of x + residual over the last dimension (hrs_layer_norm): bf16, fp16 or fp32, weight and bias fp32
         [N], statistics in fp32, one rounding.  Rows may lie at any stride; out may be x or residual."""
-        if x.dtype not in _TYPES:
-            raise ValueError(f"x must be bfloat16, float16 or float32, not {x.dtype}")
-        x2 = self._rows("x", x, x.dtype)
-        m, n = x2.shape
-        r = None
+        dtype = x.dtype
+        if dtype not in _TYPES:
+            raise ValueError(f"x must be bfloat16, float16 or float32, not {dtype}")
+        if x.dim() < 1:
+            raise ValueError("x has no dimension to normalise over")
+        n = x.shape[-1]
+        x2 = self._matrix("x", x, dtype, n)
+        r, ldr = None, 0
         if residual is not None:
-            self._check("residual", residual, x.dtype, tuple(x.shape))
-            r = self._rows("residual", residual, x.dtype)
-        if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=self.device)
-        else:
-            self._check("out", out, x.dtype, tuple(x.shape))
-        o = self._rows("out", out, x.dtype)
-        N.check(
-            N.lib().hrs_layer_norm(self._ctx, _TYPES[x.dtype], x2.data_ptr(), x2.stride(0), r.data_ptr() if r is not None else None, r.stride(0) if r is not None else 0,
-                                   self._vector("weight", weight, n), self._vector("bias", bias, n), float(eps), o.data_ptr(), o.stride(0), m, n, self._queue()),
-            "hrs_layer_norm",
-        )
+            if residual.shape != x.shape:
+                self._check("residual", residual, dtype, tuple(x.shape))
+            r2 = self._matrix("residual", residual, dtype, n)
+            r, ldr = r2.data_ptr(), r2.stride(0)
+        out = self._result(out, x.shape, dtype)
+        o = self._matrix("out", out, dtype, n)
+        rc = N.lib().hrs_layer_norm(self._ctx, _TYPES[dtype], x2.data_ptr(), x2.stride(0), r, ldr, self._vector("weight", weight, n), self._vector("bias", bias, n), eps, o.data_ptr(), o.stride(0),
+                                    x2.shape[0], n, self._queue())
+        N.check(rc, "hrs_layer_norm")
         return out
-
-    def _ints(self, name, t, n):
-        if t is None:
-            return None
-        self._check(name, t, torch.int32, (n,))
-        if n > 1 and t.stride(0) != 1:
-            raise ValueError(f"{name} must be contiguous")
-        return t.data_ptr()
 
     def attention(self, q, k, v, q_offs=None, k_offs=None, q_lens=None, k_lens=None, prefix_lens=None, causal=False, scale=None, softcap=0.0,
                   slopes=None, bias_table=None, max_q=None, max_k=None, out=None):
@@ -555,64 +559,65 @@ class Engine:
         Packed: q [T, Hq, D], k and v [Tk, Hkv, D] with q_offs int32 [B + 1] (document b is the rows q_offs[b] .. q_offs[b + 1]),
         k_offs likewise (q_offs where not given).  Padded: q [B, Sq, Hq, D], k and v [B, Sk, Hkv, D], with the number of
         valid tokens of every document in q_lens / k_lens (int32 [B]; all where not given); queries behind q_lens give
-        zeros.  Query head h reads key head h // (Hq // Hkv).  The last query of a document stands at its last key; `causal` hides the
-        keys behind a query, except the first prefix_lens[b] (int32 [B]).  Scores are scale q . k (scale D ** -0.5 where
-        not given), capped to softcap tanh(. / softcap), with a bias by distance: -slopes[h] |j - p|, or
+        zeros.  Query head h reads key head h // (Hq // Hkv).  The last query of a document stands at its last key; `causal`
+        hides the keys behind a query, except the first prefix_lens[b] (int32 [B]).  Scores are scale q . k (scale
+        D ** -0.5 where not given), capped to softcap tanh(. / softcap), with a bias by distance: -slopes[h] |j - p|, or
         bias_table[h, clamp(j - p, -R, R) + R] (fp32 [Hq, 2 R + 1]).  A query that sees no key gives zeros.
         max_q and max_k (longest documents of a packed batch) only shape the launch.  -> as q, contiguous."""
-        if q.dtype not in (torch.bfloat16, torch.float16):
-            raise ValueError(f"q must be bfloat16 or float16, not {q.dtype}")
+        dtype = q.dtype
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"q must be bfloat16 or float16, not {dtype}")
         packed = q_offs is not None
         nd = 3 if packed else 4
+        strides = []
         for name, t in (("q", q), ("k", k), ("v", v)):
-            self._check(name, t, q.dtype)
+            if t.dtype is not dtype or t.device != self.device:
+                self._check(name, t, dtype)
             if t.dim() != nd:
                 raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {'[tokens, heads, dim] (packed)' if packed else '[documents, tokens, heads, dim]'}")
-            if t.stride(-1) != 1 and t.shape[-1] > 1:
-                raise ValueError(f"{name}: the elements of a head must be next to each other (last stride {t.stride(-1)})")
-        if k.shape != v.shape or k.shape[-1] != q.shape[-1] or (not packed and k.shape[0] != q.shape[0]):
-            raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit each other or q {tuple(q.shape)}")
+            st = t.stride()
+            if st[-1] != 1 and t.shape[-1] > 1:
+                raise ValueError(f"{name}: the elements of a head must be next to each other (last stride {st[-1]})")
+            strides += (0,) + st[:2] if packed else st[:3]
+        qs, ks = q.shape, k.shape
+        if ks != v.shape or ks[-1] != qs[-1] or (not packed and ks[0] != qs[0]):
+            raise ValueError(f"k {tuple(ks)} and v {tuple(v.shape)} do not fit each other or q {tuple(qs)}")
         if packed:
             batch = q_offs.numel() - 1
             if k_offs is None:
                 k_offs = q_offs
-                if k.shape[0] != q.shape[0]:
-                    raise ValueError(f"{k.shape[0]} key tokens for {q.shape[0]} query tokens: k_offs is needed")
+                if ks[0] != qs[0]:
+                    raise ValueError(f"{ks[0]} key tokens for {qs[0]} query tokens: k_offs is needed")
         else:
-            batch = q.shape[0]
+            batch = qs[0]
             if k_offs is not None:
                 raise ValueError("k_offs needs q_offs (packed documents)")
-        a = N.AttentionArgsC()
-        a.dtype, a.batch, a.q_heads, a.kv_heads, a.head_dim = _TYPES[q.dtype], batch, q.shape[-2], k.shape[-2], q.shape[-1]
-        a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-        a.q_stride[:], a.k_stride[:], a.v_stride[:] = (((0,) + t.stride()[:2] if packed else t.stride()[:3]) for t in (q, k, v))
-        a.q_rows, a.k_rows = q.shape[-3], k.shape[-3]
-        a.q_offs, a.k_offs = self._ints("q_offs", q_offs, batch + 1), self._ints("k_offs", k_offs, batch + 1)
-        a.q_lens, a.k_lens, a.prefix_lens = self._ints("q_lens", q_lens, batch), self._ints("k_lens", k_lens, batch), self._ints("prefix_lens", prefix_lens, batch)
-        a.causal, a.softcap = int(bool(causal)), float(softcap)
-        a.scale = float(scale) if scale is not None else q.shape[-1] ** -0.5 if q.shape[-1] else 1.0
-        a.slopes = self._vector("slopes", slopes, q.shape[-2])
+        heads, dim = qs[-2], qs[-1]
+        table, reach = None, 0
         if bias_table is not None:
-            if bias_table.dim() != 2 or bias_table.shape[0] != q.shape[-2] or bias_table.shape[1] % 2 == 0 or not bias_table.is_contiguous():
-                raise ValueError(f"bias_table: shape {tuple(bias_table.shape)}, expected contiguous [{q.shape[-2]}, 2 R + 1]")
+            if bias_table.dim() != 2 or bias_table.shape[0] != heads or bias_table.shape[1] % 2 == 0 or not bias_table.is_contiguous():
+                raise ValueError(f"bias_table: shape {tuple(bias_table.shape)}, expected contiguous [{heads}, 2 R + 1]")
             self._check("bias_table", bias_table, torch.float32)
-            a.bias_table, a.bias_reach = bias_table.data_ptr(), bias_table.shape[1] // 2
-        a.max_q, a.max_k = max_q or 0, max_k or 0
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        else:
-            self._check("out", out, q.dtype, tuple(q.shape))
-            if not out.is_contiguous():
-                raise ValueError("out must be contiguous")
-        a.out = out.data_ptr()
-        L = N.lib()
+            table, reach = bias_table.data_ptr(), bias_table.shape[1] // 2
+        out = self._result(out, qs, dtype)
+        if not out.is_contiguous():
+            raise ValueError("out must be contiguous")
+        i32 = torch.int32
+        pointers = (self._vector("q_offs", q_offs, batch + 1, i32), self._vector("k_offs", k_offs, batch + 1, i32), self._vector("q_lens", q_lens, batch, i32),
+                    self._vector("k_lens", k_lens, batch, i32), self._vector("prefix_lens", prefix_lens, batch, i32), self._vector("slopes", slopes, heads), table)
+        if scale is None:
+            scale = dim**-0.5 if dim else 1.0
+        fields = [q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _TYPES[dtype], batch, heads, ks[-2], dim, 1 if causal else 0, scale, softcap, reach, *strides, qs[-3], ks[-3],
+                  *[p or 0 for p in pointers], max_q or 0, max_k or 0, 0, 0]
+        L, args = N.lib(), N.ATTENTION_ARGS.pack(*fields)
         need = C.c_size_t()
-        N.check(L.hrs_attention_workspace(self._ctx, C.byref(a), C.byref(need)), "hrs_attention_workspace")
+        N.check(L.hrs_attention_workspace(self._ctx, args, C.byref(need)), "hrs_attention_workspace")
         if need.value:
             # from torch's allocator, on the current stream: two calls, or two captured graphs, never share it
             workspace = torch.empty(need.value, dtype=torch.uint8, device=self.device)
-            a.workspace, a.workspace_bytes = workspace.data_ptr(), need.value
-        N.check(L.hrs_attention(self._ctx, C.byref(a), self._queue()), "hrs_attention")
+            fields[-2:] = workspace.data_ptr(), need.value
+            args = N.ATTENTION_ARGS.pack(*fields)
+        N.check(L.hrs_attention(self._ctx, args, self._queue()), "hrs_attention")
         return out
 
     # ---- synthetic inputs ----------------------------------------------------------------------

@@ -123,6 +123,16 @@ def test_attention_refusals(entry):
         assert L.hrs_attention_workspace(CTX, C.byref(_attention_args()), None) == ERR_ARG
 
 
+def test_attention_arguments_are_packed_as_the_header_lays_them_out():
+    """Engine.attention packs hrs_attention_args in one go: the same bytes as the structure filled field by field."""
+    a = _attention_args(softcap=3.0, bias_reach=7, q_offs=11 << 33, prefix_lens=5, bias_table=9, max_q=1 << 40, max_k=3, workspace=77, workspace_bytes=1 << 35)
+    flat = []
+    for name, _ in N.AttentionArgsC._fields_:
+        v = getattr(a, name)
+        flat += list(v) if hasattr(v, "__len__") else [v or 0]
+    assert bytes(a) == N.ATTENTION_ARGS.pack(*flat)
+
+
 def test_wrapper_refuses_host_tensors():
     eng = object.__new__(Engine)
     eng.device, eng._ctx = torch.device("cuda", 0), None
