@@ -42,6 +42,7 @@ EXPORTS = [
     "hrs_encoder_load",
     "hrs_encoder_release",
     "hrs_encode",
+    "hrs_encode_packed",
     "hrs_linear",
     "hrs_attention",
     "hrs_attention_workspace",
@@ -135,6 +136,7 @@ def lib():
             "hrs_attention": ([vp, vp, vp], i32),
             "hrs_attention_workspace": ([vp, vp, C.POINTER(C.c_size_t)], i32),
             "hrs_layer_norm": ([vp, i32, vp, i64, vp, i64, vp, vp, C.c_float, vp, i64, i64, i64, vp], i32),
+            "hrs_encode_packed": ([vp, vp, vp, vp, i32, i64, i64, vp, vp], i32),
             "hrs_row_mask_update": ([vp, i64, vp, vp, i32, i32, vp, i32, vp, vp], i32),
             "hrs_postings_register": ([vp, vp, vp, i64, i64, C.POINTER(vp)], i32),
             "hrs_postings_release": ([vp, vp], i32),

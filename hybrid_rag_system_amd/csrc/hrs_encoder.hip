@@ -1279,6 +1279,7 @@ struct hrs_encoder {
     } layer[16];
     std::vector<void*> owned;
     hrs_workspace ws;
+    hrs_encoder_any* any = nullptr;  // another geometry: everything else here is unused
 };
 
 static int dev_alloc(hrs_encoder* e, void** p, size_t bytes) {
@@ -1308,9 +1309,21 @@ static int conv_bf16(hrs_encoder* e, __bf16* dst, const float* src_dev, size_t n
 extern "C" int hrs_encoder_load(hrs_ctx* ctx, const hrs_encoder_config* cfg, const float* const* w, void* stream,
                                 hrs_encoder** out) {
     HRS_REQUIRE(ctx && cfg && w && out, "hrs_encoder_load: null argument");
-    HRS_REQUIRE(cfg->hidden == ENC_H && cfg->heads == ENC_HEADS, "hrs_encoder_load: only hidden=384, heads=12 (MiniLM-L6/L12 geometry) is built");
-    HRS_REQUIRE(cfg->inter % G_BN == 0 && cfg->inter % G_BK == 0 && cfg->inter <= 3072, "hrs_encoder_load: intermediate size %d must be a multiple of 192", cfg->inter);
-    HRS_REQUIRE(cfg->layers >= 1 && cfg->layers <= 16, "hrs_encoder_load: layers=%d outside [1,16]", cfg->layers);
+    const bool built = cfg->hidden == ENC_H && cfg->heads == ENC_HEADS && cfg->inter > 0 && cfg->inter % G_BN == 0 && cfg->inter % G_BK == 0 && cfg->inter <= 8 * ENC_H &&
+                       cfg->layers >= 1 && cfg->layers <= 16;
+    if (!built) {
+        HRS_REQUIRE(cfg->layers >= 1 && cfg->layers <= 256, "hrs_encoder_load: layers=%d outside [1, 256]", cfg->layers);
+        for (int t = 0; t < 5 + 16 * cfg->layers; ++t) HRS_REQUIRE(w[t] != nullptr, "hrs_encoder_load: weight tensor %d is null", t);
+        HRS_CHECK_HIP(hipSetDevice(ctx->device));
+        hrs_encoder_any* any = nullptr;
+        const int rc = hrs_encoder_any_load(ctx, cfg, w, stream, &any);
+        if (rc) return rc;
+        hrs_encoder* e = new hrs_encoder();
+        e->cfg = *cfg;
+        e->any = any;
+        *out = e;
+        return HRS_OK;
+    }
     HRS_REQUIRE(cfg->vocab > 0 && cfg->max_pos >= 32, "hrs_encoder_load: bad vocabulary / position table size");
     const int nt = 5 + 16 * cfg->layers;
     for (int t = 0; t < nt; ++t) HRS_REQUIRE(w[t] != nullptr, "hrs_encoder_load: weight tensor %d is null", t);
@@ -1379,6 +1392,7 @@ extern "C" int hrs_encoder_release(hrs_ctx* ctx, hrs_encoder* e) {
     (void)hipDeviceSynchronize();
     for (void* p : e->owned) (void)hipFree(p);
     if (e->ws.ptr) (void)hipFree(e->ws.ptr);
+    if (e->any) hrs_encoder_any_release(e->any);
     delete e;
     return HRS_OK;
 }
@@ -1454,6 +1468,11 @@ extern "C" int hrs_encode(hrs_ctx* ctx, hrs_encoder* e, const int32_t* ids_dev, 
                           float* out_dev, void* stream) {
     HRS_REQUIRE(ctx && e && ids_dev && lens_dev && out_dev, "hrs_encode: null argument");
     HRS_REQUIRE(B >= 1, "hrs_encode: B=%d < 1", B);
+    if (e->any) {
+        HRS_REQUIRE(S >= 1 && S <= e->cfg.max_pos && (int64_t)B * S < (1ll << 30), "hrs_encode: B=%d, S=%d (at most %d positions)", B, S, e->cfg.max_pos);
+        HRS_CHECK_HIP(hipSetDevice(ctx->device));
+        return hrs_encoder_any_run(ctx, e->any, ids_dev, nullptr, lens_dev, B, S, (int64_t)B * S, S, out_dev, (hipStream_t)stream);
+    }
     HRS_REQUIRE(S >= 32 && S <= 256 && S % 32 == 0 && S <= e->cfg.max_pos, "hrs_encode: S=%d must be a multiple of 32 in [32, 256]", S);
     HRS_CHECK_HIP(hipSetDevice(ctx->device));
     hipStream_t st = (hipStream_t)stream;
@@ -1581,4 +1600,17 @@ extern "C" int hrs_encode(hrs_ctx* ctx, hrs_encoder* e, const int32_t* ids_dev, 
     }
     HRS_CHECK_HIP(hipGetLastError());
     return HRS_OK;
+}
+
+extern "C" int hrs_encode_packed(hrs_ctx* ctx, hrs_encoder* e, const int32_t* ids_dev, const int32_t* offs_dev, int B, int64_t T, int64_t max_len, float* out_dev, void* stream) {
+    HRS_REQUIRE(ctx && e && ids_dev && offs_dev && out_dev, "hrs_encode_packed: null argument");
+    HRS_REQUIRE(B >= 1 && T >= 1 && T < (1ll << 30), "hrs_encode_packed: B=%d, T=%lld", B, (long long)T);
+    if (!e->any) {
+        hrs_set_error("hrs_encode_packed: an encoder of this geometry (hidden=%d, heads=%d) takes padded batches (hrs_encode)", e->cfg.hidden, e->cfg.heads);
+        return HRS_ERR_UNSUPPORTED;
+    }
+    HRS_CHECK_HIP(hipSetDevice(ctx->device));
+    int64_t longest = max_len > 0 ? max_len : (2 * T + B - 1) / B;
+    if (longest > T) longest = T;
+    return hrs_encoder_any_run(ctx, e->any, ids_dev, offs_dev, nullptr, B, 0, T, longest, out_dev, (hipStream_t)stream);
 }

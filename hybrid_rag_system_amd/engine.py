@@ -144,7 +144,8 @@ class InvertedPostings:
 
 
 class Encoder:
-    """MiniLM-class encoder resident on the GPU (owns its weight copies)."""
+    """Sentence encoder resident on the GPU (owns its weight copies): hidden 384 with 12 heads on kernels of its own, other
+    geometries on the engine's linear / attention / layer_norm operators."""
 
     def __init__(self, engine, weights, cfg):
         from .weights import tensor_specs
@@ -163,7 +164,8 @@ class Encoder:
         self._h = h
 
     def encode_ids(self, ids, lens):
-        """ids int32 [B,S] (S a multiple of 32, <= 256), lens int32 [B] -> fp32 [B, hidden] unit rows."""
+        """ids int32 [B,S] (S a multiple of 32, <= 256; other geometries: any S up to max_pos), lens int32 [B] -> fp32
+        [B, hidden] unit rows."""
         if not (ids.is_cuda and ids.dtype == torch.int32 and ids.dim() == 2 and ids.is_contiguous()):
             raise ValueError("ids must be a contiguous int32 [B, S] CUDA tensor")
         if not (lens.is_cuda and lens.dtype == torch.int32 and lens.numel() == ids.shape[0]):
@@ -171,6 +173,21 @@ class Encoder:
         B, S = ids.shape
         out = torch.empty((B, self.cfg.hidden), dtype=torch.float32, device=self.engine.device)
         N.check(N.lib().hrs_encode(self.engine._ctx, self._h, _ptr(ids), _ptr(lens), B, S, _ptr(out), _stream()), "hrs_encode")
+        return out
+
+    def encode_packed(self, ids, offs, max_len=0):
+        """Texts back to back, without padding: ids int32 [T], text b = ids[offs[b] : offs[b + 1]] (offs int32 [B + 1]);
+        max_len only shapes the launch -> fp32 [B, hidden] unit rows.  Not for hidden 384 with 12 heads."""
+        for name, t in (("ids", ids), ("offs", offs)):
+            if not (t.is_cuda and t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous()):
+                raise ValueError(f"{name} must be a contiguous int32 CUDA vector")
+        if offs.numel() < 1:
+            raise ValueError("offs needs one more entry than there are texts")
+        B, T = offs.numel() - 1, ids.numel()
+        out = torch.empty((B, self.cfg.hidden), dtype=torch.float32, device=self.engine.device)
+        if B == 0 or T == 0:
+            return out.zero_()
+        N.check(N.lib().hrs_encode_packed(self.engine._ctx, self._h, _ptr(ids), _ptr(offs), B, T, int(max_len), _ptr(out), _stream()), "hrs_encode_packed")
         return out
 
     def close(self):

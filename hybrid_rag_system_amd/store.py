@@ -39,7 +39,8 @@ class HrsEmbeddingFunction:
     (scripts/chromadb_helper.py:64-66): tokenise on the host, encode on the GPU, unit-norm rows.
 
     model_dir (or $HRS_MODEL_DIR) may hold `vocab.txt` + `model.safetensors` of a MiniLM-L6 class
-    model; without it the generated weights and the hash tokeniser are used (no hub access exists).
+    model, or of a BERT of another geometry with its `config.json`; without it the generated weights
+    and the hash tokeniser are used (no hub access exists).
     """
 
     def __init__(self, model_name="all-MiniLM-L6-v2", model_dir=None, seed=2026, batch_size=1024):
@@ -47,6 +48,7 @@ class HrsEmbeddingFunction:
         self.cfg = W.EncoderConfig()
         model_dir = model_dir or os.environ.get("HRS_MODEL_DIR")
         if model_dir and os.path.exists(os.path.join(model_dir, "model.safetensors")):
+            self.cfg = W.EncoderConfig.from_dir(model_dir)
             weights = W.load_safetensors(model_dir, self.cfg)
             self.tokenizer = WordPieceTokenizer(os.path.join(model_dir, "vocab.txt"))
             self.source = model_dir
@@ -58,7 +60,7 @@ class HrsEmbeddingFunction:
         self.batch_size = batch_size
 
     def embed_tensor(self, texts):
-        """-> fp32 [len(texts), 384] CUDA tensor."""
+        """-> fp32 [len(texts), hidden] CUDA tensor."""
         eng = engine()
         n = len(texts)
         if n == 0:
@@ -68,7 +70,13 @@ class HrsEmbeddingFunction:
         parts = []
         for s in range(0, n, self.batch_size):
             ids, lens = self.tokenizer.encode_batch([texts[i] for i in order[s : s + self.batch_size]])
-            parts.append(self.encoder.encode_ids(torch.from_numpy(ids).to(eng.device), torch.from_numpy(lens).to(eng.device)))
+            if self.cfg.packs:  # no padding: the texts' tokens back to back
+                offs = np.zeros(len(lens) + 1, np.int32)
+                np.cumsum(lens, out=offs[1:])
+                flat = ids[np.arange(ids.shape[1])[None, :] < lens[:, None]]
+                parts.append(self.encoder.encode_packed(torch.from_numpy(flat).to(eng.device), torch.from_numpy(offs).to(eng.device), int(lens.max())))
+            else:
+                parts.append(self.encoder.encode_ids(torch.from_numpy(ids).to(eng.device), torch.from_numpy(lens).to(eng.device)))
         emb = parts[0] if len(parts) == 1 else torch.cat(parts)
         if n == 1:
             return emb

@@ -11,6 +11,7 @@ Tensor order (101 tensors, the order of `hrs_weights` in include/hrs.h):
   q_w [H,H], q_b, k_w, k_b, v_w, v_b, o_w [H,H], o_b, ln1_g, ln1_b, i_w [I,H], i_b [I], d_w [H,I], d_b, ln2_g, ln2_b
 Linear weights are [out, in] (y = x @ w.T + b), as BERT stores them.
 """
+import json
 import os
 from dataclasses import dataclass
 
@@ -27,6 +28,27 @@ class EncoderConfig:
     max_pos: int = 512
     eps: float = 1e-12
     max_seq: int = 256  # sentence-transformers truncates all-MiniLM-L6-v2 inputs to 256 tokens
+
+    @property
+    def packs(self):
+        """Whether the encoder takes texts back to back (Encoder.encode_packed): every geometry but the built-in one."""
+        return not (self.hidden == 384 and self.heads == 12 and self.inter % 192 == 0 and self.inter <= 8 * 384 and self.layers <= 16)
+
+    @classmethod
+    def from_dir(cls, path):
+        """The geometry a local model directory names in its `config.json` (BERT's keys); without that file, or without a
+        key, the default's."""
+        file = os.path.join(path, "config.json")
+        if not os.path.exists(file):
+            return cls()
+        with open(file, encoding="utf-8") as f:
+            raw = json.load(f)
+        keys = {"vocab": "vocab_size", "hidden": "hidden_size", "layers": "num_hidden_layers", "heads": "num_attention_heads", "inter": "intermediate_size",
+                "max_pos": "max_position_embeddings", "eps": "layer_norm_eps"}
+        for key, want in (("model_type", "bert"), ("hidden_act", "gelu"), ("position_embedding_type", "absolute")):
+            if raw.get(key, want) != want:
+                raise ValueError(f"{file}: {key} {raw[key]!r} is not the encoder built here ({want})")
+        return cls(**{ours: type(getattr(cls, ours))(raw[theirs]) for ours, theirs in keys.items() if theirs in raw})
 
 
 def tensor_specs(cfg):

@@ -190,7 +190,9 @@ int hrs_profile_read(hrs_ctx* ctx, double* total_ms, int64_t* launches);
 /* Replaces the embedding function the reference builds with
  * SentenceTransformerEmbeddingFunction(model_name="all-MiniLM-L6-v2") (scripts/chromadb_helper.py:58-71)
  * and that ChromaDB calls inside collection.add / collection.query: BERT-style post-LN encoder,
- * erf-GELU, masked mean pooling, L2 normalisation.  Built for hidden = 384, heads = 12. */
+ * erf-GELU, masked mean pooling, L2 normalisation.  hidden = 384, heads = 12 (inter a multiple of 192, at most 16
+ * layers) has kernels of its own; other geometries (hidden a multiple of 8 up to 4096, heads of a multiple of 8 up to
+ * 256 wide) run on the operators of an encoder layer below. */
 typedef struct hrs_encoder_config {
     int vocab, hidden, layers, heads, inter, max_pos;
     float eps;
@@ -204,9 +206,15 @@ int hrs_encoder_load(hrs_ctx* ctx, const hrs_encoder_config* cfg, const float* c
                      hrs_encoder** out);
 int hrs_encoder_release(hrs_ctx* ctx, hrs_encoder* enc);
 /* ids_dev int32 [B, S] token ids (padded), lens_dev int32 [B] valid tokens per row, S a multiple of
- * 32 in [32, 256]; out_dev fp32 [B, hidden] unit-norm sentence embeddings. */
+ * 32 in [32, 256] (hidden 384, 12 heads) or any S up to max_pos (other geometries); out_dev fp32 [B, hidden] unit-norm
+ * sentence embeddings (other geometries: zeros for a row without tokens). */
 int hrs_encode(hrs_ctx* ctx, hrs_encoder* enc, const int32_t* ids_dev, const int32_t* lens_dev, int B, int S,
                float* out_dev, void* stream);
+/* The same for B texts back to back, without padding: text b is ids_dev[offs_dev[b] .. offs_dev[b + 1]) (int32 [B + 1],
+ * cut to the T ids); max_len: a hint of the longest (0 = unknown).  Tokens behind max_pos keep the last position.  Other
+ * geometries than hidden 384 with 12 heads; that one is HRS_ERR_UNSUPPORTED. */
+int hrs_encode_packed(hrs_ctx* ctx, hrs_encoder* enc, const int32_t* ids_dev, const int32_t* offs_dev, int B, int64_t T,
+                      int64_t max_len, float* out_dev, void* stream);
 
 /* ---- operators of an encoder layer --------------------------------------------------------- */
 /* What the forward pass behind SentenceTransformerEmbeddingFunction (scripts/chromadb_helper.py:58-71) is made of, for

@@ -142,6 +142,20 @@ def test_wrapper_refuses_host_tensors():
             call()
 
 
+def test_geometry_of_a_model_directory(tmp_path):
+    from hybrid_rag_system_amd import weights as W
+
+    assert W.EncoderConfig.from_dir(str(tmp_path)) == W.EncoderConfig() and not W.EncoderConfig().packs
+    f = tmp_path / "config.json"
+    f.write_text('{"model_type": "bert", "hidden_size": 1024, "num_attention_heads": 16, "num_hidden_layers": 24, "intermediate_size": 4096, "hidden_act": "gelu"}')
+    cfg = W.EncoderConfig.from_dir(str(tmp_path))
+    assert (cfg.hidden, cfg.heads, cfg.layers, cfg.inter, cfg.vocab, cfg.eps) == (1024, 16, 24, 4096, 30522, 1e-12) and cfg.packs
+    for bad in ('{"model_type": "t5"}', '{"hidden_act": "relu"}', '{"position_embedding_type": "relative_key"}'):
+        f.write_text(bad)
+        with pytest.raises(ValueError, match="not the encoder"):
+            W.EncoderConfig.from_dir(str(tmp_path))
+
+
 def test_oracle_bounds_hold_for_a_plain_evaluation_and_catch_mistakes():
     """The bounds the GPU tests use, on the CPU: an fp32 evaluation rounded once keeps them, small planted mistakes (a
     key too many, a wrong alignment of the last query, the residual inside the activation) do not."""
