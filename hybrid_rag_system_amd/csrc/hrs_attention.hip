@@ -238,21 +238,23 @@ __device__ __forceinline__ int swizzle_v(int i) { return DP == 32 ? i & 2 : (i &
 
 // A row of the tile and what it is allowed to see.
 struct RowPlace {
-    int64_t row;  // row / group: token, row % group: head of this key head's group
+    int row;  // row / group: token, row % group: head of this key head's group
     bool live;
     int token, head, pos, lim;
 };
+// (a division costs some 30 instructions even in 32 bits)
+__device__ __forceinline__ int token_of(const AttnArgs& a, int row) { return a.group == 1 ? row : (int)((unsigned)row / (unsigned)a.group); }
 __device__ __forceinline__ int limit_of(const AttnArgs& a, const DocRange& d, int pos, int prefix) {
     if (!a.causal) return d.lk;
     const int lim = pos + 1 > prefix ? pos + 1 : prefix;
     return lim < 0 ? 0 : lim > d.lk ? d.lk : lim;
 }
-__device__ __forceinline__ RowPlace row_place(const AttnArgs& a, const DocRange& d, int hk, int prefix, int64_t row) {
+__device__ __forceinline__ RowPlace row_place(const AttnArgs& a, const DocRange& d, int hk, int prefix, int row) {
     RowPlace r;
     r.row = row;
-    r.live = row < (int64_t)d.lq * a.group;
-    r.token = (int)(row / a.group);
-    r.head = hk * a.group + (int)(row % a.group);
+    r.live = row < d.lq * a.group;
+    r.token = token_of(a, row);
+    r.head = hk * a.group + (row - r.token * a.group);
     r.pos = r.token + d.lk - d.lq;
     r.lim = r.live ? limit_of(a, d, r.pos, prefix) : 0;
     return r;
@@ -268,22 +270,23 @@ struct Attend {
     static constexpr bool RAMP = BIAS == BIAS_SLOPE && !CAP && DP <= 64;
     x8 qf[NS];
     f32x16 acc[ND];
-    f32x16 up[RAMP ? NB : 1], down[RAMP ? NB : 1];
+    f32x16 ramp;  // before the positions; negated once the tiles have come behind them (tiles are taken in order)
+    bool flipped;
     float m, l, slope2, edge_lo, edge_hi;
     int pos, lim;
     int pos_min, pos_max, lim_min, lim_max;  // over the wave's live rows
     int table_at;                            // of the row's head in the LDS copy, at distance 0
     bool tame;                               // biases are of a size that scores do not vanish beside
 
-    __device__ __forceinline__ void open(const AttnArgs& a, const DocRange& d, int b, int hk, int prefix, int64_t row0, const RowPlace& r, const float* table) {
+    __device__ __forceinline__ void open(const AttnArgs& a, const DocRange& d, int b, int hk, int prefix, int row0, const RowPlace& r, const float* table) {
         const int lane = threadIdx.x & 63, h = lane >> 5;
         const T* qp = (const T*)a.q + b * a.q_sb + (d.q0 + r.token) * a.q_st + r.head * a.q_sh + h * 8;
 #pragma unroll
         for (int s = 0; s < NS; ++s) qf[s] = (r.live && s * 16 + h * 8 < a.dim) ? *(const x8*)(qp + s * 16) : (x8)((T)0.f);
-        const int64_t rows = (int64_t)d.lq * a.group, last = row0 + 31 < rows - 1 ? row0 + 31 : rows - 1;
-        pos_min = (int)(row0 / a.group) + d.lk - d.lq;
-        pos_max = (int)(last / a.group) + d.lk - d.lq;
+        const int rows = d.lq * a.group, last = row0 + 31 < rows - 1 ? row0 + 31 : rows - 1;
         const bool any = row0 < rows;
+        pos_min = token_of(a, row0) + d.lk - d.lq;
+        pos_max = (any ? token_of(a, last) : 0) + d.lk - d.lq;
         lim_min = any ? limit_of(a, d, pos_min, prefix) : 0;
         lim_max = any ? limit_of(a, d, pos_max, prefix) : 0;
         pos_min = __builtin_amdgcn_readfirstlane(pos_min);
@@ -301,12 +304,8 @@ struct Attend {
             const float per = slope2 / a.scale2;
             tame = !__any(!(fabsf(per) < 1e15f));
 #pragma unroll
-            for (int n = 0; n < NB; ++n)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    up[n][e] = per * (float)(n * 32 + 8 * (e >> 2) + (e & 3));
-                    down[n][e] = -up[n][e];
-                }
+            for (int e = 0; e < 16; ++e) ramp[e] = per * (float)(8 * (e >> 2) + (e & 3));
+            flipped = false;
         }
         if constexpr (BIAS == BIAS_TABLE) {
             table_at = (r.head - hk * a.group) * (2 * a.reach + 1) + a.reach;
@@ -330,16 +329,20 @@ struct Attend {
     // Keys j0 .. j0 + KT - 1, of which those below lim are seen; kl, vl: their tile in LDS.
     __device__ __forceinline__ void tile(const AttnArgs& a, const char* kl, const char* vl, const float* table, int j0) {
         const int lane = threadIdx.x & 63, h = lane >> 5, c32 = lane & 31;
-        const bool before = tame && j0 + KT - 1 <= pos_min, behind = tame && j0 >= pos_max;  // (of a slope)
+        const bool before = tame && j0 + KT - 1 <= pos_min, behind = tame && !before && j0 >= pos_max;  // (of a slope)
+        if constexpr (RAMP) {
+            if (behind && !flipped) {
+                ramp = -ramp;
+                flipped = true;
+            }
+        }
         f32x16 s[NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
             const int i = n * 32 + c32;
             if constexpr (RAMP) {
-                if (before)
-                    s[n] = mfma32(*(const x8*)(kl + i * (DP * 2) + ((h ^ swizzle_k<DP>(i)) << 4)), qf[0], up[n]);
-                else if (behind)
-                    s[n] = mfma32(*(const x8*)(kl + i * (DP * 2) + ((h ^ swizzle_k<DP>(i)) << 4)), qf[0], down[n]);
+                if (before || behind)
+                    s[n] = mfma32(*(const x8*)(kl + i * (DP * 2) + ((h ^ swizzle_k<DP>(i)) << 4)), qf[0], ramp);
                 else
                     s[n] = mfma32(*(const x8*)(kl + i * (DP * 2) + ((h ^ swizzle_k<DP>(i)) << 4)), qf[0], (f32x16)(0.f));
             } else {
@@ -355,8 +358,8 @@ struct Attend {
             asm volatile("s_nop 11");
             __builtin_amdgcn_sched_barrier(0);
         }
-        // x = s mul + add is the score in base 2
-        float mul = CAP ? 1.f : a.scale2, add = 0.f;
+        // x = s mul + add + n more is the score in base 2 (n: the tile's 32 keys)
+        float mul = CAP ? 1.f : a.scale2, add = 0.f, more = 0.f;
         const int d0 = j0 + 4 * h - pos;  // distance of this lane's first key
         if constexpr (CAP) {
 #pragma unroll
@@ -367,8 +370,10 @@ struct Attend {
         if constexpr (BIAS == BIAS_SLOPE) {
             if (RAMP && before) {
                 add = slope2 * (float)d0;
+                more = slope2 * 32.f;
             } else if (RAMP && behind) {
                 add = -slope2 * (float)d0;
+                more = slope2 * -32.f;
             } else {
 #pragma unroll
                 for (int n = 0; n < NB; ++n)
@@ -402,15 +407,25 @@ struct Attend {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[n][e] = n * 32 + 8 * (e >> 2) + (e & 3) < left ? s[n][e] : -INFINITY;
         }
+        float off[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) off[n] = RAMP ? fmaf((float)n, more, add) : add;
         if constexpr (!FIXED) {
-            float top = s[0][0];
+            float top = -INFINITY;
 #pragma unroll
-            for (int n = 0; n < NB; ++n)
+            for (int n = 0; n < NB; ++n) {
+                float t[4] = {s[n][0], s[n][1], s[n][2], s[n][3]};  // (four chains: a maximum waits for the one before)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) top = fmaxf(top, s[n][e]);
-            top = fmaf(top, mul, add);
+                for (int e = 4; e < 16; e += 4)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) t[i] = fmaxf(t[i], s[n][e + i]);
+                top = fmaxf(top, fmaf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), mul, off[n]));
+            }
             top = fmaxf(top, swap_halves(top));
-            if (__any(top > m)) {  // (in a long row the maximum rarely moves after the first tiles)
+            // The base m of a row's weights follows its maximum only when that is 2^8 ahead: weights up to 256 are as exact
+            // as those up to 1 (fp16's largest is 65504), and the sums need not be rescaled each time some row of the
+            // wave finds a new maximum, which over 8192 keys of random scores is in three tiles of five.
+            if (__any(top > m + 8.f)) {
                 const float m_new = fmaxf(m, top);
                 const float keep = exp2_hw(m - (m_new == -INFINITY ? 0.f : m_new));
                 m = m_new;
@@ -418,17 +433,25 @@ struct Attend {
 #pragma unroll
                 for (int i = 0; i < ND; ++i) acc[i] *= keep;
             }
-            add -= m == -INFINITY ? 0.f : m;  // nothing seen so far: every weight is exp2(-inf) = 0
+            const float base = m == -INFINITY ? 0.f : m;  // nothing seen so far: every weight is exp2(-inf) = 0
+#pragma unroll
+            for (int n = 0; n < NB; ++n) off[n] -= base;
         }
+        // The sum of weights is that of the rounded ones, two per instruction: numerator and denominator round alike.
         x8 pf[2 * NB];
+        float part[4] = {l, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float w = FIXED ? exp2_hw(s[n][e]) : exp2_hw(fmaf(s[n][e], mul, add));
-                l += w;
-                pf[2 * n + (e >> 3)][e & 7] = (T)w;
+            for (int e = 0; e < 16; e += 2) {
+                const float w0 = FIXED ? exp2_hw(s[n][e]) : exp2_hw(fmaf(s[n][e], mul, off[n]));
+                const float w1 = FIXED ? exp2_hw(s[n][e + 1]) : exp2_hw(fmaf(s[n][e + 1], mul, off[n]));
+                const typename vec_of<T>::x2 w = {(T)w0, (T)w1};
+                part[(e >> 1) & 3] = add_pair(w, part[(e >> 1) & 3]);
+                pf[2 * n + (e >> 3)][e & 7] = w[0];
+                pf[2 * n + (e >> 3)][(e & 7) + 1] = w[1];
             }
+        l = (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
         for (int t = 0; t < 2 * NB; ++t)
 #pragma unroll
@@ -547,7 +570,7 @@ __device__ __forceinline__ float inverse(float l) { return l > 0.f || l != l ? 1
 // ---- many rows: 128 per workgroup, 32 per wave ---------------------------------------------------------
 // All four waves read the tiles of 64 keys (32 for heads wider than 128) that they fetch together, two buffers deep.
 template <typename T, int DP, int BIAS, bool CAP, bool FIXED>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attend_rows(AttnArgs a) {
+__global__ __launch_bounds__(256, DP <= 64 && !(BIAS == BIAS_SLOPE && !CAP) ? 3 : DP <= 128 ? 2 : 1) void k_attend_rows(AttnArgs a) {
     constexpr int NB = DP <= 128 ? 2 : 1, KT = NB * 32, TILE = KT * DP * 2;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const float* table = (const float*)(lds + 4 * TILE);
@@ -559,7 +582,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attend_rows(AttnArgs
     id /= a.tiles;
     const int hk = id % a.kv_heads, b = id / a.kv_heads;
     const DocRange dr = doc_range(a, b);
-    const int64_t rows = (int64_t)dr.lq * a.group, rows_all = (int64_t)dr.q_total * a.group;
+    const int rows = dr.lq * a.group, rows_all = dr.q_total * a.group;
     const T* kbase = (const T*)a.k + b * a.k_sb + dr.k0 * a.k_st + hk * a.k_sh;
     const T* vbase = (const T*)a.v + b * a.v_sb + dr.k0 * a.v_st + hk * a.v_sh;
     const int prefix = a.prefix ? a.prefix[b] : 0;
@@ -573,15 +596,16 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attend_rows(AttnArgs
     load.open(a, wv);
     const uint32_t l0 = lds_addr_of(lds);
 
-    for (int64_t row0 = (int64_t)t0 * 128; row0 < rows_all; row0 += (int64_t)a.tiles * 128) {
+    // (a row number stays below 2^31: at most 2^29 rows, and steps of at most 2^29 + 128)
+    for (int row0 = t0 * 128; row0 < rows_all; row0 += a.tiles * 128) {
         const RowPlace r = row_place(a, dr, hk, prefix, row0 + wv * 32 + (lane & 31));
         Attend<T, DP, NB, BIAS, CAP, FIXED> st;
         st.open(a, dr, b, hk, prefix, row0 + wv * 32, r, table);
         // keys that any row of the workgroup sees
         int need = 0;
         if (row0 < rows) {
-            const int64_t last = row0 + 127 < rows - 1 ? row0 + 127 : rows - 1;
-            need = limit_of(a, dr, (int)(last / a.group) + dr.lk - dr.lq, prefix);
+            const int last = row0 + 127 < rows - 1 ? row0 + 127 : rows - 1;
+            need = limit_of(a, dr, token_of(a, last) + dr.lk - dr.lq, prefix);
             if (need > from + a.chunk) need = from + a.chunk;
         }
         int buf = 0;
@@ -598,7 +622,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attend_rows(AttnArgs
             store_row<T>(a, st.acc, inverse(st.l), orow, write);
         else
             store_part(a, st.acc, st.m, st.l, chunk, orow, write);
-        if (row0 + (int64_t)a.tiles * 128 < rows_all) __syncthreads();  // (the next rows fetch over the last tile)
+        if (row0 + a.tiles * 128 < rows_all) __syncthreads();  // (the next rows fetch over the last tile)
     }
 }
 
@@ -616,7 +640,7 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(AttnArgs a) {
     id /= a.kv_heads;
     const int chunk = id % a.chunks, b = id / a.chunks;
     const DocRange dr = doc_range(a, b);
-    const int64_t rows_all = (int64_t)dr.q_total * a.group;
+    const int rows_all = dr.q_total * a.group;
     const T* kbase = (const T*)a.k + b * a.k_sb + dr.k0 * a.k_st + hk * a.k_sh;
     const T* vbase = (const T*)a.v + b * a.v_sb + dr.k0 * a.v_st + hk * a.v_sh;
     const int prefix = a.prefix ? a.prefix[b] : 0;
@@ -631,7 +655,7 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(AttnArgs a) {
     char* mine = lds + wv * RING;
     const uint32_t l0 = lds_addr_of(lds) + wv * RING;
 
-    for (int64_t row0 = 0; row0 < rows_all; row0 += 32) {
+    for (int row0 = 0; row0 < rows_all; row0 += 32) {
         const RowPlace r = row_place(a, dr, hk, prefix, row0 + (lane & 31));
         Attend<T, DP, 1, BIAS, CAP, FIXED> st;
         st.open(a, dr, b, hk, prefix, row0, r, table);
@@ -692,40 +716,51 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(AttnArgs a) {
 }
 
 // ---- the chunks of a row joined --------------------------------------------------------------------------
-// One wave per row: o = sum_c o_c 2^(m_c - m) / sum_c l_c 2^(m_c - m), chunks in order.
+// One workgroup per row: o = sum_c o_c 2^(m_c - m) / sum_c l_c 2^(m_c - m).  Thread (phase, piece) adds the chunks phase,
+// phase + phases, .. of its 4 dimensions; the phases meet in LDS in order.
 template <typename T>
 __global__ __launch_bounds__(256) void k_attend_join(AttnArgs a, int rows_hint) {
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    const int groups = (rows_hint + 3) / 4;
-    const int b = blockIdx.x / groups;
+    __shared__ float factor[256], wave_top[4], wave_sum[4];
+    __shared__ f32x4 sums[256];
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const int b = blockIdx.x / rows_hint;
     const DocRange dr = doc_range(a, b);
     const int64_t rows_all = (int64_t)dr.q_total * a.heads;
-    const int n = dr.lk <= a.chunk ? 1 : (dr.lk + a.chunk - 1) / a.chunk;
-    for (int64_t row = (int64_t)(blockIdx.x % groups) * 4 + wv; row < rows_all; row += (int64_t)groups * 4) {
+    const int n = dr.lk <= a.chunk ? 1 : (dr.lk + a.chunk - 1) / a.chunk;  // at most 256
+    const int pieces = a.dim / 4, phases = 256 / pieces, ph = tid / pieces, d = (tid - ph * pieces) * 4;
+    for (int64_t row = blockIdx.x % rows_hint; row < rows_all; row += rows_hint) {
         const int64_t at = ((a.q_offs ? 0 : b * a.q_rows) + dr.q0) * a.heads + row;
-        float m = -INFINITY;
-        for (int c = 0; c < n; ++c) m = fmaxf(m, a.part_ml[c * a.part_rows + at].x);
-        const float base = m == -INFINITY ? 0.f : m;
-        float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-        const int d = lane * 4;
-        for (int c = 0; c < n; ++c) {
-            const float2 ml = a.part_ml[c * a.part_rows + at];
-            const float f = exp2_hw(ml.x - base);
-            l += ml.y * f;
-            if (d < a.dim) {
-                const f32x4 v = *(const f32x4*)(a.part + (c * a.part_rows + at) * a.dim + d);
+        const float2 ml = tid < n ? a.part_ml[tid * a.part_rows + at] : make_float2(-INFINITY, 0.f);
+        float m = ml.x;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] += v[e] * f;
-            }
+        for (int x = 32; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+        if (lane == 0) wave_top[wv] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
+        const float f = exp2_hw(ml.x - (m == -INFINITY ? 0.f : m));
+        factor[tid] = f;
+        float l = ml.y * f;
+#pragma unroll
+        for (int x = 32; x > 0; x >>= 1) l += __shfl_xor(l, x);
+        if (lane == 0) wave_sum[wv] = l;
+        __syncthreads();
+        l = (wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3]);
+        f32x4 o = (f32x4)(0.f);
+        if (ph < phases) {
+#pragma unroll 4
+            for (int c = ph; c < n; c += phases) o += *(const f32x4*)(a.part + (c * a.part_rows + at) * a.dim + d) * factor[c];
         }
-        const float inv = inverse(l);
-        if (d < a.dim) {
-            T* op = (T*)a.out + at * a.dim + d;
+        sums[tid] = o;
+        __syncthreads();
+        if (ph == 0) {
+            for (int p = 1; p < phases; ++p) o += sums[p * pieces + tid];
+            const float inv = inverse(l);
             T v[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = (T)(o[e] * inv);
-            __builtin_memcpy(op, v, 8);
+            __builtin_memcpy((T*)a.out + at * a.dim + d, v, 8);
         }
+        __syncthreads();
     }
 }
 
@@ -793,9 +828,9 @@ static int launch_type(hrs_ctx* ctx, const AttnArgs& a, const AttnPlan& p, hipSt
     else
         rc = launch_dim<T, 256>(ctx, a, p, st);
     if (rc || a.chunks == 1) return rc;
-    const int64_t rows = p.longest_q * a.heads, groups = (rows + 3) / 4;
-    HRS_REQUIRE(rows < (1ll << 30) && groups * a.batch < (1ll << 31), "hrs_attention: %lld rows to join", (long long)rows);
-    hipLaunchKernelGGL(k_attend_join<T>, dim3((unsigned)(groups * a.batch)), dim3(256), 0, st, a, (int)rows);
+    int64_t rows = p.longest_q * a.heads;  // workgroups per document
+    if (rows > (1 << 20) / a.batch + 1) rows = (1 << 20) / a.batch + 1;
+    hipLaunchKernelGGL(k_attend_join<T>, dim3((unsigned)(rows * a.batch)), dim3(256), 0, st, a, (int)rows);
     HRS_CHECK_HIP(hipGetLastError());
     return HRS_OK;
 }
@@ -807,6 +842,7 @@ static int attention_args(const hrs_attention_args* p, AttnArgs& a) {
     HRS_REQUIRE(p->head_dim >= 8 && p->head_dim <= 256 && p->head_dim % 8 == 0, "hrs_attention: head_dim=%d must be a multiple of 8 in [8, 256]", p->head_dim);
     HRS_REQUIRE(p->q_rows >= 0 && p->k_rows >= 0 && p->q_rows < (1ll << 30) && p->k_rows < (1ll << 30), "hrs_attention: q_rows=%lld, k_rows=%lld",
                 (long long)p->q_rows, (long long)p->k_rows);
+    HRS_REQUIRE(p->q_rows * (p->q_heads / p->kv_heads) <= (1ll << 29), "hrs_attention: q_rows=%lld with %d query heads per key head", (long long)p->q_rows, p->q_heads / p->kv_heads);
     HRS_REQUIRE(p->scale > 0.f && p->scale < INFINITY, "hrs_attention: scale=%g must be positive and finite", (double)p->scale);
     HRS_REQUIRE(p->softcap >= 0.f && p->softcap < INFINITY, "hrs_attention: softcap=%g must be finite, 0 for none", (double)p->softcap);
     HRS_REQUIRE(!(p->slopes && p->bias_table), "hrs_attention: slopes and bias_table exclude each other");
@@ -876,7 +912,7 @@ static AttnPlan plan_attention(hrs_ctx* ctx, const hrs_attention_args* p, AttnAr
     if (!plan.fast) return plan;
     plan.few = rows <= 32;
     // Too few workgroups for the card: long documents are cut into chunks of keys, joined by a second launch.
-    const int64_t groups = (int64_t)a.batch * a.kv_heads * (plan.few ? 1 : a.tiles), want = 4 * (int64_t)ctx->num_cu;
+    const int64_t groups = (int64_t)a.batch * a.kv_heads * (plan.few ? 1 : a.tiles), want = (plan.few ? 8 : 4) * (int64_t)ctx->num_cu;
     if (groups < want / 2 && longest_k > 1024) {
         int64_t chunks = want / groups, most = longest_k / 512;
         if (chunks > most) chunks = most;

@@ -16,11 +16,13 @@ template <>
 struct vec_of<__bf16> {
     typedef __bf16 x8 __attribute__((ext_vector_type(8)));
     typedef __bf16 x4 __attribute__((ext_vector_type(4)));
+    typedef __bf16 x2 __attribute__((ext_vector_type(2)));
 };
 template <>
 struct vec_of<_Float16> {
     typedef _Float16 x8 __attribute__((ext_vector_type(8)));
     typedef _Float16 x4 __attribute__((ext_vector_type(4)));
+    typedef _Float16 x2 __attribute__((ext_vector_type(2)));
 };
 
 // D[16 rows of a][16 rows of b] += a b^T over 32 of the depth: lane l gives row l % 16, depth (l / 16) * 8 .. + 7 of either
@@ -31,6 +33,16 @@ __device__ __forceinline__ f32x4 mfma16(vec_of<_Float16>::x8 a, vec_of<_Float16>
 // 8 g + 4 (l / 32) + i (register 4 g + i) of column l % 32.
 __device__ __forceinline__ f32x16 mfma32(vec_of<__bf16>::x8 a, vec_of<__bf16>::x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mfma32(vec_of<_Float16>::x8 a, vec_of<_Float16>::x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+// c + v[0] + v[1] in fp32
+__device__ __forceinline__ float add_pair(vec_of<__bf16>::x2 v, float c) {
+    const vec_of<__bf16>::x2 one = {(__bf16)1.f, (__bf16)1.f};
+    return __builtin_amdgcn_fdot2_f32_bf16(v, one, c, false);
+}
+__device__ __forceinline__ float add_pair(vec_of<_Float16>::x2 v, float c) {
+    const vec_of<_Float16>::x2 one = {(_Float16)1.f, (_Float16)1.f};
+    return __builtin_amdgcn_fdot2(v, one, c, false);
+}
 
 // Every earlier load of this wave has arrived, every earlier LDS access of it is done; then the workgroup's barrier.
 __device__ __forceinline__ void wait_all_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }

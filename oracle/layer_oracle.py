@@ -132,6 +132,7 @@ def attention(q, k, v, lq, lk, causal=False, prefix=None, scale=None, cap=0.0, s
         tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
         spread = p @ vh.abs()
         mean_rel = (p * rel).sum(-1, keepdim=True)
-        err = (p * rel) @ vh.abs() + (u + mean_rel + 4 * (lk + 64) * F) * spread + (seen.double() @ vh.abs()) * tiny / torch.where(some, total, torch.ones_like(total))
+        # (weights w (1 + d), |d| <= u, in numerator and denominator alike move o by sum p d (v - o), at most u (spread + |o|))
+        err = (p * rel) @ vh.abs() + (u + mean_rel + 4 * (lk + 64) * F) * (spread + o[:lq, h].abs()) + (seen.double() @ vh.abs()) * tiny / torch.where(some, total, torch.ones_like(total))
         bound[:lq, h] = _rounded(o[:lq, h], dtype) + (1 + 4 * u) * err
     return o, bound
