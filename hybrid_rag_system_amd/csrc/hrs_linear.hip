@@ -99,7 +99,7 @@ __device__ __forceinline__ TilePos tile_at(int id, int tm, int tn) {
 template <typename T, int BM, int BN, int WR, int WC, int ACT>
 __global__ __launch_bounds__(64 * WR * WC, 2) void k_linear_any(LinearArgs a) {
     typedef typename vec_of<T>::x8 x8;
-    constexpr int NTHR = 64 * WR * WC, MT = BM / WR / 16, NT = BN / WC / 16, STAGE = (BM + BN) * 128;
+    constexpr int NTHR = 64 * WR * WC, MT = BM / WR / 16, NT = BN / WC / 16;
     constexpr int PX = BM * 8 / NTHR, PW = BN * 8 / NTHR;  // pieces a thread moves per stage
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, qd = lane >> 4, r16 = lane & 15;
@@ -135,9 +135,9 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void k_linear_any(LinearArgs a) {
         for (int j = 0; j < NT; ++j) acc[i][j] = (f32x4)(0.f);
     if (stages) fetch(0);
     for (int s = 0; s < stages; ++s) {
-        char* buf = lds + (s & 1) * STAGE;  // (its contents of two stages ago were read before the barrier of stage s - 1)
+        __syncthreads();  // the stage before has been read
 #pragma unroll
-        for (int j = 0; j < PX + PW; ++j) *(x8*)(buf + at[j]) = in[j];
+        for (int j = 0; j < PX + PW; ++j) *(x8*)(lds + at[j]) = in[j];
         __syncthreads();
         if (s + 1 < stages) fetch(s + 1);
 #pragma unroll
@@ -146,12 +146,12 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void k_linear_any(LinearArgs a) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 const int row = wn + feature_of(t, r16);
-                wf[t] = *(const x8*)(buf + (BM + row) * 128 + (((t2 * 4 + qd) ^ key_w(row)) << 4));
+                wf[t] = *(const x8*)(lds + (BM + row) * 128 + (((t2 * 4 + qd) ^ key_w(row)) << 4));
             }
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 const int row = wm + i * 16 + r16;
-                const x8 xf = *(const x8*)(buf + row * 128 + (((t2 * 4 + qd) ^ key_x(row)) << 4));
+                const x8 xf = *(const x8*)(lds + row * 128 + (((t2 * 4 + qd) ^ key_x(row)) << 4));
 #pragma unroll
                 for (int t = 0; t < NT; ++t) acc[i][t] = mfma16(wf[t], xf, acc[i][t]);
             }
@@ -502,7 +502,7 @@ static int launch_few(const LinearArgs& a, bool aligned, hipStream_t st) {
 template <typename T, int BM, int BN, int WR, int WC, int ACT>
 static int launch_any(hrs_ctx* ctx, const LinearArgs& a, hipStream_t st) {
     static hrs_per_device_once attr;
-    const int lds = 2 * (BM + BN) * 128;
+    const int lds = (BM + BN) * 128;
     const auto kernel = k_linear_any<T, BM, BN, WR, WC, ACT>;
     if (attr.need(ctx->device)) {
         HRS_CHECK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
@@ -522,8 +522,9 @@ static int launch_linear(hrs_ctx* ctx, const LinearArgs& a, hipStream_t st) {
     auto tiles = [&](int bm, int bn) { return (a.M + bm - 1) / bm * ((a.N + bn - 1) / bn); };
     const int64_t cus = ctx->num_cu;
     if (!aligned || a.K == 0) {
-        // Measured at K = 773 (us): 1000 x 1000: 10.2 with 64 x 64 tiles, 13.0 with 128 x 64, 13.9 with 128 x 128;
-        // 4999 x 1537, where 128 x 128 leaves eight tiles for a second round: 42.9, 40.1, 43.9;  8192 x 2048: 71, 57, 45.
+        // Measured at K = 773 (us): 1000 x 1001: 9.5 with 64 x 64 tiles, 12.6 with 128 x 64, 14.9 with 128 x 128;
+        // 4999 x 1537, where 128 x 128 leaves eight tiles for a second round: 43.5, 37.0, 44.6 (4999 x 1536, which does not:
+        // 38.9, 31.5, 23.6);  8192 x 2047: 80, 66, 56.
         if (tiles(64, 64) <= 2 * cus) return launch_any<T, 64, 64, 2, 2, ACT>(ctx, a, st);
         const int64_t t = tiles(128, 128), rounds = (t + 2 * cus - 1) / (2 * cus);
         if (10 * t < 6 * rounds * 2 * cus) return launch_any<T, 128, 64, 2, 2, ACT>(ctx, a, st);
