@@ -23,6 +23,7 @@ struct AttnArgs {
     int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;  // strides in elements: document, token, head
     int64_t q_rows, k_rows;  // tokens per document, or of all documents where offsets are given
     int batch, heads, kv_heads, group, dim, tiles;
+    int b0;  // first document of this launch
     int causal, reach;
     float scale2;        // scale log2 e
     float cap2, cap_in;  // cap log2 e; 2 log2 e scale / cap
@@ -110,7 +111,7 @@ __global__ __launch_bounds__(256) void k_attend_any(AttnArgs a) {
     int id = blockIdx.x;
     const int t0 = id % a.tiles;
     id /= a.tiles;
-    const int hk = id % a.kv_heads, b = id / a.kv_heads;
+    const int hk = id % a.kv_heads, b = a.b0 + id / a.kv_heads;
     const DocRange dr = doc_range(a, b);
     const int64_t rows = (int64_t)dr.lq * a.group, rows_all = (int64_t)dr.q_total * a.group;
     const T* kbase = (const T*)a.k + b * a.k_sb + dr.k0 * a.k_st + hk * a.k_sh;
@@ -580,7 +581,7 @@ __global__ __launch_bounds__(256, DP <= 64 && !(BIAS == BIAS_SLOPE && !CAP) ? 3 
     id /= a.chunks;
     const int t0 = a.tiles - 1 - id % a.tiles;  // causal: the longest rows first
     id /= a.tiles;
-    const int hk = id % a.kv_heads, b = id / a.kv_heads;
+    const int hk = id % a.kv_heads, b = a.b0 + id / a.kv_heads;
     const DocRange dr = doc_range(a, b);
     const int rows = dr.lq * a.group, rows_all = dr.q_total * a.group;
     const T* kbase = (const T*)a.k + b * a.k_sb + dr.k0 * a.k_st + hk * a.k_sh;
@@ -638,7 +639,7 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(AttnArgs a) {
     int id = spread_over_xcds((int)blockIdx.x, (int)gridDim.x);
     const int hk = id % a.kv_heads;
     id /= a.kv_heads;
-    const int chunk = id % a.chunks, b = id / a.chunks;
+    const int chunk = id % a.chunks, b = a.b0 + id / a.chunks;
     const DocRange dr = doc_range(a, b);
     const int rows_all = dr.q_total * a.group;
     const T* kbase = (const T*)a.k + b * a.k_sb + dr.k0 * a.k_st + hk * a.k_sh;
@@ -723,7 +724,7 @@ __global__ __launch_bounds__(256) void k_attend_join(AttnArgs a, int rows_hint) 
     __shared__ float factor[256], wave_top[4], wave_sum[4];
     __shared__ f32x4 sums[256];
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    const int b = blockIdx.x / rows_hint;
+    const int b = a.b0 + blockIdx.x / rows_hint;
     const DocRange dr = doc_range(a, b);
     const int64_t rows_all = (int64_t)dr.q_total * a.heads;
     const int n = dr.lk <= a.chunk ? 1 : (dr.lk + a.chunk - 1) / a.chunk;  // at most 256
@@ -775,7 +776,7 @@ struct AttnPlan {
 
 template <typename K>
 static int launch_attend(hrs_ctx* ctx, hrs_per_device_once& attr, K kernel, int threads, int lds, int64_t grid, const AttnArgs& a, hipStream_t st) {
-    HRS_REQUIRE(grid < (1ll << 31), "hrs_attention: %lld workgroups", (long long)grid);
+    HRS_REQUIRE(grid < (1 << 24), "hrs_attention: %lld workgroups for one document", (long long)grid);
     if (lds > 65536 && attr.need(ctx->device)) {
         HRS_CHECK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
         attr.done(ctx->device);
@@ -829,7 +830,7 @@ static int launch_type(hrs_ctx* ctx, const AttnArgs& a, const AttnPlan& p, hipSt
         rc = launch_dim<T, 256>(ctx, a, p, st);
     if (rc || a.chunks == 1) return rc;
     int64_t rows = p.longest_q * a.heads;  // workgroups per document
-    if (rows > (1 << 20) / a.batch + 1) rows = (1 << 20) / a.batch + 1;
+    if (rows > (1 << 20) / a.batch + 1) rows = (1 << 20) / a.batch + 1;  // (each takes further rows in turn)
     hipLaunchKernelGGL(k_attend_join<T>, dim3((unsigned)(rows * a.batch)), dim3(256), 0, st, a, (int)rows);
     HRS_CHECK_HIP(hipGetLastError());
     return HRS_OK;
@@ -985,5 +986,13 @@ extern "C" int hrs_attention(hrs_ctx* ctx, const hrs_attention_args* p, void* st
     }
     hrs_device_scope dev(ctx->device);
     HRS_CHECK_HIP(dev.err);
-    return p->dtype == HRS_TYPE_BF16 ? launch_type<__bf16>(ctx, a, plan, (hipStream_t)stream) : launch_type<_Float16>(ctx, a, plan, (hipStream_t)stream);
+    // as many documents per launch as a grid holds (less than 2^32 threads)
+    const int64_t each = (int64_t)a.kv_heads * a.chunks * (plan.few ? 1 : a.tiles), most = each < (1 << 23) ? (1 << 23) / each : 1;
+    for (int b0 = 0; b0 < p->batch; b0 += (int)most) {
+        a.b0 = b0;
+        a.batch = p->batch - b0 < most ? p->batch - b0 : (int)most;
+        rc = p->dtype == HRS_TYPE_BF16 ? launch_type<__bf16>(ctx, a, plan, (hipStream_t)stream) : launch_type<_Float16>(ctx, a, plan, (hipStream_t)stream);
+        if (rc) return rc;
+    }
+    return HRS_OK;
 }

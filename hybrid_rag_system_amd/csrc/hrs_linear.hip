@@ -572,20 +572,26 @@ extern "C" int hrs_linear(hrs_ctx* ctx, int dtype, const void* x_dev, int64_t ld
     HRS_REQUIRE(y_dev != x_dev && y_dev != w_dev, "hrs_linear: y may not be x or W");
     HRS_REQUIRE(((uintptr_t)x_dev | (uintptr_t)w_dev | (uintptr_t)y_dev | (uintptr_t)resid_dev) % 2 == 0 && (uintptr_t)bias_dev % 4 == 0,
                 "hrs_linear: an operand is not aligned to its elements");
+    HRS_REQUIRE(resid_dev != y_dev || ldr == ldy || M == 1, "hrs_linear: y in place of the residual needs its row stride (%lld, not %lld)", (long long)ldr, (long long)ldy);
     hrs_device_scope dev(ctx->device);
     HRS_CHECK_HIP(dev.err);
     LinearArgs a;
-    a.x = x_dev;
     a.w = w_dev;
     a.bias = bias_dev;
-    a.resid = resid_dev;
-    a.y = y_dev;
     a.ldx = ldx;
     a.ldw = ldw;
     a.ldr = ldr;
     a.ldy = ldy;
-    a.M = M;
     a.N = (int)N;
     a.K = (int)K;
-    return dtype == HRS_TYPE_BF16 ? launch_linear_act<__bf16>(ctx, a, act, (hipStream_t)stream) : launch_linear_act<_Float16>(ctx, a, act, (hipStream_t)stream);
+    const int64_t most = 1 << 22;  // rows per launch: a grid holds less than 2^32 threads
+    for (int64_t m0 = 0; m0 < M; m0 += most) {
+        a.x = (const char*)x_dev + m0 * ldx * 2;
+        a.y = (char*)y_dev + m0 * ldy * 2;
+        a.resid = resid_dev ? (const char*)resid_dev + m0 * ldr * 2 : nullptr;
+        a.M = M - m0 < most ? M - m0 : most;
+        const int rc = dtype == HRS_TYPE_BF16 ? launch_linear_act<__bf16>(ctx, a, act, (hipStream_t)stream) : launch_linear_act<_Float16>(ctx, a, act, (hipStream_t)stream);
+        if (rc) return rc;
+    }
+    return HRS_OK;
 }

@@ -164,18 +164,23 @@ static int launch_norm(const NormArgs& a, hipStream_t st) {
 int hrs_launch_norm(int dtype, const void* x, int64_t ldx, const void* resid, int64_t ldr, const float* gamma, const float* beta,
                     float eps, void* y, int64_t ldy, int64_t M, int N, hipStream_t st) {
     NormArgs a;
-    a.x = x;
-    a.resid = resid;
     a.gamma = gamma;
     a.beta = beta;
-    a.y = y;
     a.ldx = ldx;
     a.ldr = ldr;
     a.ldy = ldy;
-    a.M = M;
     a.N = N;
     a.eps = eps;
-    return dtype == HRS_TYPE_BF16 ? launch_norm<__bf16>(a, st) : dtype == HRS_TYPE_FP16 ? launch_norm<_Float16>(a, st) : launch_norm<float>(a, st);
+    const int64_t most = 1 << 22, el = dtype == HRS_TYPE_FP32 ? 4 : 2;  // rows per launch: a grid holds less than 2^32 threads
+    for (int64_t m0 = 0; m0 < M; m0 += most) {
+        a.x = (const char*)x + m0 * ldx * el;
+        a.resid = resid ? (const char*)resid + m0 * ldr * el : nullptr;
+        a.y = (char*)y + m0 * ldy * el;
+        a.M = M - m0 < most ? M - m0 : most;
+        const int rc = dtype == HRS_TYPE_BF16 ? launch_norm<__bf16>(a, st) : dtype == HRS_TYPE_FP16 ? launch_norm<_Float16>(a, st) : launch_norm<float>(a, st);
+        if (rc) return rc;
+    }
+    return HRS_OK;
 }
 
 extern "C" int hrs_layer_norm(hrs_ctx* ctx, int dtype, const void* x_dev, int64_t ldx, const void* resid_dev, int64_t ldr,
@@ -192,6 +197,7 @@ extern "C" int hrs_layer_norm(hrs_ctx* ctx, int dtype, const void* x_dev, int64_
     const uintptr_t el = dtype == HRS_TYPE_FP32 ? 4 : 2;
     HRS_REQUIRE(((uintptr_t)x_dev | (uintptr_t)y_dev | (uintptr_t)resid_dev) % el == 0 && ((uintptr_t)gamma_dev | (uintptr_t)beta_dev) % 4 == 0,
                 "hrs_layer_norm: an operand is not aligned to its elements");
+    HRS_REQUIRE((x_dev != y_dev || ldx == ldy || M == 1) && (resid_dev != y_dev || ldr == ldy || M == 1), "hrs_layer_norm: y in place of x or r needs its row stride");
     hrs_device_scope dev(ctx->device);
     HRS_CHECK_HIP(dev.err);
     return hrs_launch_norm(dtype, x_dev, ldx, resid_dev, ldr, gamma_dev, beta_dev, eps, y_dev, ldy, M, (int)N, (hipStream_t)stream);

@@ -227,7 +227,7 @@ enum hrs_activation { HRS_ACT_NONE = 0, HRS_ACT_RELU = 1, HRS_ACT_GELU = 2 /* er
 /* y = act(x W^T + b) + r: x [M, K], W [N, K], r (nullable) and y [M, N] of type dtype (bf16 or fp16), rows ld* elements
  * apart, elements of a row next to each other; bias (nullable) fp32 [N].  Sums, bias, activation and residual in fp32,
  * one rounding at the end.  Any sizes, strides and alignments; rows of 16-byte aligned operands with strides and K that
- * are multiples of 8 take the fastest kernels.  y may be r (element by element), not x or W.  K = 0 gives act(b) + r. */
+ * are multiples of 8 take the fastest kernels.  y may be r (with the same stride), not x or W.  K = 0 gives act(b) + r. */
 int hrs_linear(hrs_ctx* ctx, int dtype, const void* x_dev, int64_t ldx, const void* w_dev, int64_t ldw,
                const float* bias_dev, const void* resid_dev, int64_t ldr, int act, void* y_dev, int64_t ldy, int64_t M,
                int64_t N, int64_t K, void* stream);
@@ -270,7 +270,7 @@ int hrs_attention_workspace(hrs_ctx* ctx, const hrs_attention_args* args, size_t
 
 /* y = (z - mean z) / sqrt(var z + eps) * gamma + beta with z = x + r, row by row: x, r (nullable) and y [M, N] of type
  * dtype (bf16, fp16 or fp32), rows ld* elements apart; gamma and beta (nullable) fp32 [N].  z, mean and variance in
- * fp32, one rounding at the end.  y may be x or r. */
+ * fp32, one rounding at the end.  y may be x or r (with the same stride). */
 int hrs_layer_norm(hrs_ctx* ctx, int dtype, const void* x_dev, int64_t ldx, const void* resid_dev, int64_t ldr,
                    const float* gamma_dev, const float* beta_dev, float eps, void* y_dev, int64_t ldy, int64_t M,
                    int64_t N, void* stream);

@@ -269,6 +269,49 @@ def test_attention_of_long_documents(eng):
     _attention_case(eng, "padded", [1111], [2222], 1, 1, 128, "fp16", True, [1700], 40.0, "table", 100, seed=2, size=3.0)
 
 
+def test_attention_table_too_large_for_lds(eng):
+    """A table of more rows than a workgroup keeps (16 KB) is read from memory."""
+    _attention_case(eng, "packed", [150, 33], [150, 33], 4, 1, 64, "bf16", bias="table", reach=2500, seed=4)
+    _attention_case(eng, "padded", [1, 1], [3000, 40], 2, 2, 32, "fp16", True, bias="table", reach=4000, seed=5)
+
+
+def test_offsets_past_32_bits(eng):
+    """Keys that start 2^31 elements into the tensor, and a product whose output is larger than that."""
+    n, h, d = 2_200_000, 8, 128
+    kv = torch.zeros((1, n, h, d), dtype=torch.bfloat16, device="cuda")
+    kv[:, -4000:] = torch.randn(1, 4000, h, d, device="cuda").bfloat16()
+    q = torch.randn(1, 1, 16, d, device="cuda").bfloat16()
+    slopes = torch.full((16,), 0.5, device="cuda")  # keys more than some hundred tokens back weigh nothing
+    got, want = eng.attention(q, kv, kv, slopes=slopes), eng.attention(q, kv[:, -4000:], kv[:, -4000:], slopes=slopes)
+    assert (got.float() - want.float()).abs().max() <= 2.0**-7 * want.float().abs().max()
+    many = torch.randn(1, 300, 8, d, device="cuda").bfloat16()
+    got, want = eng.attention(many, kv, kv, causal=True, slopes=slopes[:8]), eng.attention(many, kv[:, -4000:], kv[:, -4000:], causal=True, slopes=slopes[:8])
+    assert (got.float() - want.float()).abs().max() <= 2.0**-7 * want.float().abs().max()
+    del kv
+    m, k, n = 600_000, 64, 4096
+    x, w = torch.randn(m, k, device="cuda").bfloat16(), torch.randn(n, k, device="cuda").bfloat16()
+    y = eng.linear(x, w)
+    assert torch.equal(y[-300:], eng.linear(x[-300:], w)) and torch.equal(y[:300], eng.linear(x[:300], w))
+    y = eng.linear(x[:, :63], w[:, :63])  # the same through the kernels for any alignment
+    assert torch.equal(y[-300:], eng.linear(x[-300:, :63], w[:, :63]))
+
+
+def test_more_rows_and_documents_than_one_launch_takes(eng):
+    m = (1 << 22) + 70  # rows of 8
+    x, w = torch.randn(m, 8, device="cuda").bfloat16(), torch.randn(8, 8, device="cuda").bfloat16()
+    y = eng.linear(x, w)
+    assert torch.equal(y[-100:], eng.linear(x[-100:], w)) and torch.equal(y[:100], eng.linear(x[:100], w))
+    g = torch.ones(8, device="cuda")
+    z = eng.layer_norm(x, g)
+    assert torch.equal(z[-100:], eng.layer_norm(x[-100:], g)) and torch.equal(z[:100], eng.layer_norm(x[:100], g))
+    docs, h = 600_000, 16  # 9.6 million pairs of a document and a head
+    offs = torch.arange(docs + 1, device="cuda", dtype=torch.int32) * 2
+    q = torch.randn(2 * docs, h, 8, device="cuda").bfloat16()
+    out = eng.attention(q, q, q, q_offs=offs, max_q=2)
+    for part in (slice(0, 200), slice(2 * docs - 200, 2 * docs), slice(1048476, 1048676)):
+        assert torch.equal(out[part], eng.attention(q[part], q[part], q[part], q_offs=offs[:101], max_q=2))
+
+
 def test_attention_scores_far_apart(eng):
     """Scores in the thousands, a scale of its own, weights that are one-hot: the running maximum has to move."""
     _attention_case(eng, "padded", [90], [900], 2, 2, 64, "bf16", size=9.0, scale=1.0, seed=5)

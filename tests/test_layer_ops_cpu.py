@@ -43,6 +43,7 @@ def test_linear_refusals():
     _refused(call(y=_p(256)), "may not be x")
     for kw in ({"x": _p(1)}, {"w": _p(257)}, {"y": _p(513)}, {"r": _p(1)}, {"bias": _p(2)}):
         _refused(call(**kw), "aligned")
+    _refused(call(r=_p(512), ldr=16), "in place of the residual")
     assert call(m=0, x=None, w=None, y=None) == 0 and call(n=0, w=None, y=None) == 0  # nothing to do
 
 
@@ -63,6 +64,8 @@ def test_layer_norm_refusals():
     _refused(call(ldy=4), "overlap")
     for kw in ({"x": _p(1)}, {"dtype": 2, "y": _p(514)}, {"g": _p(258)}, {"b": _p(1)}):
         _refused(call(**kw), "aligned")
+    _refused(call(y=_p(0), ldy=16), "in place")
+    _refused(call(r=_p(512), ldr=16), "in place")
     assert call(m=0, x=None, y=None, g=None) == 0 and call(n=0, x=None, y=None, g=None) == 0
 
 
