@@ -36,6 +36,7 @@ struct AttnArgs {
 
 enum { BIAS_NONE = 0, BIAS_SLOPE = 1, BIAS_TABLE = 2 };
 #define LOG2E 1.44269504088896f
+#define TABLE_EDGE 96  // 64 keys of a tile and 32 rows of a wave
 
 struct DocRange {
     int64_t q0, k0;  // first token, from the start of the tensor
@@ -309,7 +310,7 @@ struct Attend {
             flipped = false;
         }
         if constexpr (BIAS == BIAS_TABLE) {
-            table_at = (r.head - hk * a.group) * (2 * a.reach + 1) + a.reach;
+            table_at = (r.head - hk * a.group) * (2 * (a.reach + TABLE_EDGE) + 1) + a.reach + TABLE_EDGE;
             edge_lo = table[table_at - a.reach];
             edge_hi = table[table_at + a.reach];
             tame = !__any(!(fabsf(edge_lo) < 1e30f && fabsf(edge_hi) < 1e30f));
@@ -389,13 +390,13 @@ struct Attend {
             } else if (tame && j0 >= pos_max + a.reach) {
                 add = edge_hi;
             } else {
-                const bool inner = j0 + KT - 1 - pos_min <= a.reach && j0 - pos_max >= -a.reach;
+                // a tile that reaches into the table is at most KT + 30 past its ends, which the copy in LDS repeats
 #pragma unroll
                 for (int n = 0; n < NB; ++n)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         int d = d0 + n * 32 + 8 * (e >> 2) + (e & 3);
-                        if (!inner) d = d < -a.reach ? -a.reach : d > a.reach ? a.reach : d;
+                        if (!tame) d = d < -a.reach ? -a.reach : d > a.reach ? a.reach : d;
                         s[n][e] = (CAP ? s[n][e] : s[n][e] * a.scale2) + table[table_at + d];
                     }
                 mul = 1.f;
@@ -508,11 +509,18 @@ struct TileLoad {
     }
 };
 
-// Table rows of a key head's group, in base 2 (a finite entry stays finite, also the type's lowest value).
+// Table rows of a key head's group, in base 2 (a finite entry stays finite, also the type's lowest value), each with its
+// first and last entry repeated TABLE_EDGE times.
 __device__ __forceinline__ void stage_table(const AttnArgs& a, int hk, float* dst) {
-    const int n = a.group * (2 * a.reach + 1);
-    const float* src = a.table + (int64_t)hk * n;
-    for (int i = threadIdx.x; i < n; i += blockDim.x) dst[i] = fmaxf(src[i] * LOG2E, fminf(src[i], -1e30f));
+    const int width = 2 * a.reach + 1, wide = width + 2 * TABLE_EDGE;
+    for (int g = 0; g < a.group; ++g) {
+        const float* src = a.table + (int64_t)(hk * a.group + g) * width;
+        for (int i = threadIdx.x; i < wide; i += blockDim.x) {
+            const int at = i - TABLE_EDGE;
+            const float t = src[at < 0 ? 0 : at < width ? at : width - 1];
+            dst[g * wide + i] = fmaxf(t * LOG2E, fminf(t, -1e30f));
+        }
+    }
 }
 
 __device__ __forceinline__ int64_t out_row(const AttnArgs& a, const DocRange& d, int b, int token, int head) {
@@ -589,28 +597,30 @@ __global__ __launch_bounds__(256, DP <= 64 && !(BIAS == BIAS_SLOPE && !CAP) ? 3 
     const int prefix = a.prefix ? a.prefix[b] : 0;
     const int from = chunk * a.chunk;
     if (from > 0 && from >= dr.lk) return;
+    TileLoad<DP, KT, 4> load;
+    load.open(a, wv);
+    const uint32_t l0 = lds_addr_of(lds);
+    // keys that any of the workgroup's rows from row0 on sees, in this chunk; the first tile of them is requested at once
+    auto begin = [&](int row0) __attribute__((always_inline)) {
+        if (row0 >= rows) return 0;
+        const int last = row0 + 127 < rows - 1 ? row0 + 127 : rows - 1;
+        int need = limit_of(a, dr, token_of(a, last) + dr.lk - dr.lq, prefix);
+        if (need > from + a.chunk) need = from + a.chunk;
+        if (from < need) load.issue(a, kbase, vbase, from, dr.lk, l0, l0 + TILE, wv);
+        return need;
+    };
+    int need = begin(t0 * 128);
     if constexpr (BIAS == BIAS_TABLE) {
         stage_table(a, hk, (float*)(lds + 4 * TILE));
         __syncthreads();
     }
-    TileLoad<DP, KT, 4> load;
-    load.open(a, wv);
-    const uint32_t l0 = lds_addr_of(lds);
 
     // (a row number stays below 2^31: at most 2^29 rows, and steps of at most 2^29 + 128)
     for (int row0 = t0 * 128; row0 < rows_all; row0 += a.tiles * 128) {
         const RowPlace r = row_place(a, dr, hk, prefix, row0 + wv * 32 + (lane & 31));
         Attend<T, DP, NB, BIAS, CAP, FIXED> st;
         st.open(a, dr, b, hk, prefix, row0 + wv * 32, r, table);
-        // keys that any row of the workgroup sees
-        int need = 0;
-        if (row0 < rows) {
-            const int last = row0 + 127 < rows - 1 ? row0 + 127 : rows - 1;
-            need = limit_of(a, dr, token_of(a, last) + dr.lk - dr.lq, prefix);
-            if (need > from + a.chunk) need = from + a.chunk;
-        }
         int buf = 0;
-        if (from < need) load.issue(a, kbase, vbase, from, dr.lk, l0, l0 + TILE, wv);
         for (int j0 = from; j0 < need; j0 += KT, buf ^= 1) {
             wait_all_barrier();  // the tile has landed; everyone has read the one before
             if (j0 + KT < need) load.issue(a, kbase, vbase, j0 + KT, dr.lk, l0 + (buf ^ 1) * 2 * TILE, l0 + (buf ^ 1) * 2 * TILE + TILE, wv);
@@ -623,7 +633,10 @@ __global__ __launch_bounds__(256, DP <= 64 && !(BIAS == BIAS_SLOPE && !CAP) ? 3 
             store_row<T>(a, st.acc, inverse(st.l), orow, write);
         else
             store_part(a, st.acc, st.m, st.l, chunk, orow, write);
-        if (row0 + a.tiles * 128 < rows_all) __syncthreads();  // (the next rows fetch over the last tile)
+        if (row0 + a.tiles * 128 < rows_all) {
+            __syncthreads();  // (the next rows fetch over the last tile)
+            need = begin(row0 + a.tiles * 128);
+        }
     }
 }
 
@@ -788,7 +801,7 @@ static int launch_attend(hrs_ctx* ctx, hrs_per_device_once& attr, K kernel, int 
 template <typename T, int DP, int BIAS, bool CAP, bool FIXED>
 static int launch_fast(hrs_ctx* ctx, const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
     static hrs_per_device_once once_few, once_rows;
-    const int table = BIAS == BIAS_TABLE ? a.group * (2 * a.reach + 1) * 4 : 0;
+    const int table = BIAS == BIAS_TABLE ? a.group * (2 * (a.reach + TABLE_EDGE) + 1) * 4 : 0;
     const int64_t pairs = (int64_t)a.batch * a.kv_heads;
     if (p.few) {
         constexpr int NW = DP == 256 ? 2 : 4;
@@ -909,7 +922,7 @@ static AttnPlan plan_attention(hrs_ctx* ctx, const hrs_attention_args* p, AttnAr
     const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out;
     const int64_t strides = a.q_sb | a.q_st | a.q_sh | a.k_sb | a.k_st | a.k_sh | a.v_sb | a.v_st | a.v_sh;
     plan.fast = at % 16 == 0 && strides % 8 == 0 && a.k_st < (1 << 23) && a.v_st < (1 << 23) &&
-                (!a.table || (int64_t)a.group * (2 * a.reach + 1) * 4 <= ATTN_TABLE_LDS);
+                (!a.table || (int64_t)a.group * (2 * (a.reach + TABLE_EDGE) + 1) * 4 <= ATTN_TABLE_LDS);
     if (!plan.fast) return plan;
     plan.few = rows <= 32;
     // Many documents: one workgroup takes all rows of a document (it walks on while there are rows), since most would find
