@@ -95,7 +95,10 @@ __device__ __forceinline__ TilePos tile_at(int id, int tm, int tn) {
 }
 
 
-// Any alignment: pieces pass through registers, those of the next stage while this one is multiplied.
+// Any alignment: pieces pass through registers, those of the next stage while this one is multiplied.  One LDS buffer
+// (24 or 32 KB), so that several workgroups of a CU cover each other's barriers.  Bound by the L1's rate for pieces that
+// straddle lines and by how the tiles fill the card: 4999 x 1537 x 773 takes 37 us (43 with tanh, a residual and rows of y
+// at odd addresses), 4999 x 1536 x 773, whose 128 x 128 tiles fit one round, 24 us.
 template <typename T, int BM, int BN, int WR, int WC, int ACT>
 __global__ __launch_bounds__(64 * WR * WC, 2) void k_linear_any(LinearArgs a) {
     typedef typename vec_of<T>::x8 x8;
@@ -172,7 +175,8 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void k_linear_any(LinearArgs a) {
 //
 // KG groups of WR x WC waves share the depth of one tile: each walks its own run of stages through its own ring, and the
 // first adds the sums of the others in order.  That is for products with few tiles, whose time is the latency of one
-// stage (about 0.3 us) times their number.
+// stage (about 0.3 us) times their number: 1024 x 1024 x 1024 6.7 us with the depth shared by two (7.8 without),
+// 256 x 1024 x 4096 8.7 us with 32 x 32 tiles shared by four (20.5 with 64 x 64 tiles unshared).
 template <typename T, int BM, int BN, int RING, int WR, int WC, int KG, int ACT>
 __global__ __launch_bounds__(64 * WR * WC * KG) void k_linear_tile(LinearArgs a) {
     typedef typename vec_of<T>::x8 x8;
@@ -284,6 +288,11 @@ __global__ __launch_bounds__(64 * WR * WC * KG) void k_linear_tile(LinearArgs a)
 // A half's place in LDS is free as soon as both groups have read it, and is filled again for two stages ahead in the
 // next phase: a piece has a whole stage (2048 cycles) to arrive, and every phase waits for the half that the next one
 // reads with a counted wait, 8 younger requests still in flight.
+// 8192^3: 755 us, 1.46 PFLOP/s (a large library product there: 0.69 ms, 1.58); per 1024 of depth a 65536 x 4096 product takes
+// 336 us, as the library's does, and 150 us besides: 107 of them are its 537 MB of output at the card's copy rate, which
+// nothing here runs under, since all workgroups finish their tiles at about the same time.  Workgroups that stay and fetch
+// the next tile under their stores were built and took the same time (486 us either way).  gelu adds 97 us to the 487:
+// 13 vector operations per value with the matrix pipe idle.
 template <typename T, int ACT>
 __global__ __launch_bounds__(512, 2) void k_linear_wide(LinearArgs a) {
     typedef typename vec_of<T>::x8 x8;
@@ -419,6 +428,8 @@ __global__ __launch_bounds__(512, 2) void k_linear_wide(LinearArgs a) {
 // ---- few tokens -------------------------------------------------------------------------------------------
 // Up to 16 tokens: W is read once, straight into the matrix instruction's operand (lane l: feature l % 16, 16 bytes of
 // its row), 16 features per workgroup; its 8 or 16 waves share the depth and join their sums in LDS in a fixed order.
+// Latency: 12 x 1536 x 384 2.8 us, 16 x 4096 x 1024 4.1 us (2.1 TB/s of W), 16 x 1024 x 4096 9.2 us; 32 x 32 tiles of
+// k_linear_tile: 3.5, 4.1 and 8.7 us, but those waste half of the matrix instruction and need aligned operands.
 template <typename T, int NW, bool ALIGNED, int ACT>
 __global__ __launch_bounds__(64 * NW) void k_linear_few(LinearArgs a) {
     typedef typename vec_of<T>::x8 x8;

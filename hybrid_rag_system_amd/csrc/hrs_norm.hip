@@ -61,7 +61,8 @@ __device__ __forceinline__ void store_norm(const NormArgs& a, T* y, int c, const
     }
 }
 
-// WPR waves per row, CH pieces of 8 elements per lane: rows of up to 512 CH WPR elements.
+// WPR waves per row, CH pieces of 8 elements per lane: rows of up to 512 CH WPR elements.  65536 x 1024 bf16 with a
+// residual: 70 us, 5.7 TB/s (a copy of 2 GiB reaches 4.96; part of the input is still in the 256 MB cache); 12 x 384: 2.7 us.
 template <typename T, int CH, int WPR>
 __global__ __launch_bounds__(256) void k_layer_norm(NormArgs a) {
     __shared__ float part[2][4];
