@@ -910,6 +910,7 @@ static int attention_args(const hrs_attention_args* p, AttnArgs& a) {
         a.cap2 = p->softcap * LOG2E;
         a.cap_in = 2.f * LOG2E * p->scale / p->softcap;
     }
+    HRS_REQUIRE(a.scale2 < 1e30f && a.cap2 < 1e30f && a.cap_in < 1e30f, "hrs_attention: scale=%g with softcap=%g leaves the range of fp32", (double)p->scale, (double)p->softcap);
     return HRS_OK;
 }
 

@@ -506,11 +506,14 @@ class Engine:
             raise ValueError(f"{name} must be contiguous")
         return t.data_ptr()
 
-    def _result(self, out, shape, dtype):
+    def _result(self, out, like, shape, n):
+        """-> (the result, its address, elements from row to row): `out`, or a new tensor of `shape`."""
         if out is None:
-            return torch.empty(shape, dtype=dtype, device=self.device)
-        self._check("out", out, dtype, tuple(shape))
-        return out
+            out = like.new_empty(shape)
+            return out, out.data_ptr(), n
+        self._check("out", out, like.dtype, tuple(shape))
+        o = self._matrix("out", out, like.dtype, n)
+        return out, o.data_ptr(), o.stride(0)
 
     def _queue(self):
         """The current stream of this engine's GPU (whatever the current GPU is)."""
@@ -520,7 +523,7 @@ class Engine:
         """act(x @ weight.T + bias) + residual in one kernel (hrs_linear): x [.., K] and weight [N, K] bf16 or fp16, bias
         fp32 [N], residual [.., N] as x; activation "none", "relu", "gelu" (erf), "gelu_tanh", "silu" or "tanh".  Rows may
         lie at any stride.  Sums, bias, activation and residual in fp32, one rounding.  out (as the result) may be
-        residual, not x or weight."""
+        residual, not x or weight.  Forward only."""
         dtype = x.dtype
         if dtype not in (torch.bfloat16, torch.float16):
             raise ValueError(f"x must be bfloat16 or float16, not {dtype}")
@@ -539,16 +542,14 @@ class Engine:
                 self._check("residual", residual, dtype, tuple(shape))
             r2 = self._matrix("residual", residual, dtype, n)
             r, ldr = r2.data_ptr(), r2.stride(0)
-        out = self._result(out, shape, dtype)
-        o = self._matrix("out", out, dtype, n)
-        rc = N.lib().hrs_linear(self._ctx, _TYPES[dtype], x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), self._vector("bias", bias, n), r, ldr, act, o.data_ptr(), o.stride(0), m, n, k,
-                                self._queue())
+        out, y, ldy = self._result(out, x, shape, n)
+        rc = N.lib().hrs_linear(self._ctx, _TYPES[dtype], x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), self._vector("bias", bias, n), r, ldr, act, y, ldy, m, n, k, self._queue())
         N.check(rc, "hrs_linear")
         return out
 
     def layer_norm(self, x, weight, bias=None, eps=1e-12, residual=None, out=None):
         """LayerNorm of x + residual over the last dimension (hrs_layer_norm): bf16, fp16 or fp32, weight and bias fp32
-        [N], statistics in fp32, one rounding.  Rows may lie at any stride; out may be x or residual."""
+        [N], statistics in fp32, one rounding.  Rows may lie at any stride; out may be x or residual.  Forward only."""
         dtype = x.dtype
         if dtype not in _TYPES:
             raise ValueError(f"x must be bfloat16, float16 or float32, not {dtype}")
@@ -562,10 +563,9 @@ class Engine:
                 self._check("residual", residual, dtype, tuple(x.shape))
             r2 = self._matrix("residual", residual, dtype, n)
             r, ldr = r2.data_ptr(), r2.stride(0)
-        out = self._result(out, x.shape, dtype)
-        o = self._matrix("out", out, dtype, n)
-        rc = N.lib().hrs_layer_norm(self._ctx, _TYPES[dtype], x2.data_ptr(), x2.stride(0), r, ldr, self._vector("weight", weight, n), self._vector("bias", bias, n), eps, o.data_ptr(), o.stride(0),
-                                    x2.shape[0], n, self._queue())
+        out, y, ldy = self._result(out, x, x.shape, n)
+        rc = N.lib().hrs_layer_norm(self._ctx, _TYPES[dtype], x2.data_ptr(), x2.stride(0), r, ldr, self._vector("weight", weight, n), self._vector("bias", bias, n), eps, y, ldy, x2.shape[0], n,
+                                    self._queue())
         N.check(rc, "hrs_layer_norm")
         return out
 
@@ -580,7 +580,7 @@ class Engine:
         hides the keys behind a query, except the first prefix_lens[b] (int32 [B]).  Scores are scale q . k (scale
         D ** -0.5 where not given), capped to softcap tanh(. / softcap), with a bias by distance: -slopes[h] |j - p|, or
         bias_table[h, clamp(j - p, -R, R) + R] (fp32 [Hq, 2 R + 1]).  A query that sees no key gives zeros.
-        max_q and max_k (longest documents of a packed batch) only shape the launch.  -> as q, contiguous."""
+        max_q and max_k (longest documents of a packed batch) only shape the launch.  -> as q, contiguous.  Forward only."""
         dtype = q.dtype
         if dtype not in (torch.bfloat16, torch.float16):
             raise ValueError(f"q must be bfloat16 or float16, not {dtype}")
@@ -616,9 +616,12 @@ class Engine:
                 raise ValueError(f"bias_table: shape {tuple(bias_table.shape)}, expected contiguous [{heads}, 2 R + 1]")
             self._check("bias_table", bias_table, torch.float32)
             table, reach = bias_table.data_ptr(), bias_table.shape[1] // 2
-        out = self._result(out, qs, dtype)
-        if not out.is_contiguous():
-            raise ValueError("out must be contiguous")
+        if out is None:
+            out = q.new_empty(qs)
+        else:
+            self._check("out", out, dtype, tuple(qs))
+            if not out.is_contiguous():
+                raise ValueError("out must be contiguous")
         i32 = torch.int32
         pointers = (self._vector("q_offs", q_offs, batch + 1, i32), self._vector("k_offs", k_offs, batch + 1, i32), self._vector("q_lens", q_lens, batch, i32),
                     self._vector("k_lens", k_lens, batch, i32), self._vector("prefix_lens", prefix_lens, batch, i32), self._vector("slopes", slopes, heads), table)

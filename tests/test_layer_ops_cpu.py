@@ -106,6 +106,9 @@ def test_attention_refusals(entry):
         ({"scale": float("nan")}, "scale"),
         ({"scale": float("inf")}, "scale"),
         ({"softcap": -1.0}, "softcap"),
+        ({"scale": 1e31}, "range"),
+        ({"softcap": 1e-35}, "range"),
+        ({"softcap": 1e32}, "range"),
         ({"softcap": float("nan")}, "softcap"),
         ({"slopes": ptr, "bias_table": ptr}, "exclude"),
         ({"bias_table": ptr, "bias_reach": -1}, "bias_reach"),
