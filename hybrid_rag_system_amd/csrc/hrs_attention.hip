@@ -226,7 +226,7 @@ __global__ __launch_bounds__(256) void k_attend_any(AttnArgs a) {
                     if (d < a.dim) {
                         T o[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[e] = (T)(acc[i][4 * g + e] * inv);
+                        for (int e = 0; e < 4; ++e) o[e] = live ? (T)(acc[i][4 * g + e] * inv) : (T)0.f;
                         __builtin_memcpy(op + d, o, 8);
                     }
                 }

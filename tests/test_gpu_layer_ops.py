@@ -357,6 +357,17 @@ def test_attention_nan_in_one_query_stays_there(eng):
     assert torch.equal(got, clean)
 
 
+@pytest.mark.parametrize("queries", [5, 70])
+@pytest.mark.parametrize("aligned", [True, False])
+def test_attention_queries_behind_the_last_are_zero_whatever_v_holds(eng, queries, aligned):
+    q, k, v = (torch.randn(1, n, 2, 64, device="cuda").bfloat16() for n in (queries, 90, 90))
+    v[0, 7, 0, 3], v[0, 8, 1, 4] = float("nan"), float("inf")
+    if not aligned:
+        k = torch.cat([k, k[..., :1]], -1)[..., :64]
+    got = eng.attention(q, k, v, q_lens=torch.tensor([3], dtype=torch.int32, device="cuda"))
+    assert (got[0, 3:] == 0).all() and torch.isnan(got[0, :3, 0, 3]).all() and torch.isfinite(got[0, :3, :, 5:]).all()
+
+
 def test_random_cases(eng):
     rng = random.Random(11)
     for i in range(40):
