@@ -26,7 +26,7 @@ struct AttnArgs {
     int b0;  // first document of this launch
     int causal, reach;
     float scale2;        // scale log2 e
-    float cap2, cap_in;  // cap log2 e; 2 log2 e scale / cap
+    float cap2, cap_in, cap_u;  // cap log2 e; 2 log2 e scale / cap; scale / cap
     // long documents: `chunk` keys per workgroup, unnormalised sums [chunks][rows][dim] and (m, l) [chunks][rows]
     int chunk, chunks;
     int64_t part_rows;
@@ -86,10 +86,28 @@ __device__ __forceinline__ float swap_halves(float v) {
     return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
 }
 
+// cap tanh(scale s / cap) in base 2.  tanh u = 1 - 2 / (1 + e^2u) is off by 2^-22 or so of 1 whatever u is: up to a cap of
+// 64 that is less than 2e-5 of a score.  Larger caps would lose small scores that way, so below |u| = 0.4 capped takes tanh's
+// series up to u^11 (next term 3.6e-3 u^12 < 7e-8), above it the same quotient, there within 2^-21 of its result.  Kernels
+// of their own (CAP_ANY), as a branch in the others it would cost them registers: two documents of 8192 tokens, 16 heads of
+// 64: 1085 us with a cap of 100, 912 with 60; 8 tokens over 32768 keys, 32 / 8 heads of 128: 229 and 207.
+enum { CAP_NONE = 0, CAP_TO_64 = 1, CAP_ANY = 2 };
+#define CAP_DIRECT (64.f * LOG2E)
+__device__ __forceinline__ float capped_direct(const AttnArgs& a, float s) { return fmaf(-2.f * a.cap2, rcp_hw(1.f + exp2_hw(s * a.cap_in)), a.cap2); }
+__device__ __forceinline__ float capped(const AttnArgs& a, float s) {
+    const float u = s * a.cap_u, t = u * u;
+    float p = fmaf(t, -0.0088632355f, 0.0218694885f);
+    p = fmaf(t, p, -0.0539682540f);
+    p = fmaf(t, p, 0.1333333333f);
+    p = fmaf(t, p, -0.3333333333f);
+    p = fmaf(t, p, 1.f);
+    return t < 0.16f ? s * a.scale2 * p : capped_direct(a, s);
+}
+
 // Score of one (query, key) pair in base 2: s is q . k, d = j - p_i.
 template <int BIAS, bool CAP>
 __device__ __forceinline__ float score2(const AttnArgs& a, float s, float slope2, const float* table, int d) {
-    float x = CAP ? fmaf(-2.f * a.cap2, rcp_hw(1.f + exp2_hw(s * a.cap_in)), a.cap2) : s * a.scale2;
+    float x = !CAP ? s * a.scale2 : a.cap2 > CAP_DIRECT ? capped(a, s) : capped_direct(a, s);
     if constexpr (BIAS == BIAS_SLOPE) x = fmaf(-slope2, fabsf((float)d), x);
     if constexpr (BIAS == BIAS_TABLE) {
         const int at = d < -a.reach ? -a.reach : d > a.reach ? a.reach : d;
@@ -265,7 +283,7 @@ __device__ __forceinline__ RowPlace row_place(const AttnArgs& a, const DocRange&
 }
 
 // The state of one lane's row (query c = lane % 32 of the wave; the wave's halves hold different keys and dimensions).
-template <typename T, int DP, int NB, int BIAS, bool CAP, bool FIXED>
+template <typename T, int DP, int NB, int BIAS, int CAP, bool FIXED>
 struct Attend {
     typedef typename vec_of<T>::x8 x8;
     static constexpr int ND = DP / 32, NS = DP / 16, KT = NB * 32;
@@ -369,7 +387,7 @@ struct Attend {
 #pragma unroll
             for (int n = 0; n < NB; ++n)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[n][e] = fmaf(-2.f * a.cap2, rcp_hw(1.f + exp2_hw(s[n][e] * a.cap_in)), a.cap2);
+                for (int e = 0; e < 16; ++e) s[n][e] = CAP == CAP_ANY ? capped(a, s[n][e]) : capped_direct(a, s[n][e]);
         }
         if constexpr (BIAS == BIAS_SLOPE) {
             if (RAMP && before) {
@@ -478,18 +496,16 @@ struct Attend {
 template <int DP, int KT, int NWAVES>
 struct TileLoad {
     static constexpr int PPR = DP / 8, RPI = 64 / PPR, NI = KT / RPI / NWAVES;
-    int kof[NI], vof[NI], kp[NI], vp[NI], row[NI];
+    int kof[NI], vof[NI], row0;  // this lane's row of instruction j is row0 + j RPI
     __device__ __forceinline__ void open(const AttnArgs& a, int wave) {
         const int lane = threadIdx.x & 63;
+        row0 = wave * NI * RPI + lane / PPR;
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
-            row[j] = (wave * NI + j) * RPI + lane / PPR;
-            const int pk = (lane % PPR) ^ swizzle_k<DP>(row[j]), pv = (lane % PPR) ^ swizzle_v<DP>(row[j]);
+            const int row = row0 + j * RPI, pk = (lane % PPR) ^ swizzle_k<DP>(row), pv = (lane % PPR) ^ swizzle_v<DP>(row);
             // (a piece behind the head's dimension repeats the first: it meets zeros of q, or ends in columns not stored)
-            kp[j] = pk * 8 < a.dim ? pk * 16 : 0;
-            vp[j] = pv * 8 < a.dim ? pv * 16 : 0;
-            kof[j] = row[j] * (int)(a.k_st * 2) + kp[j];
-            vof[j] = row[j] * (int)(a.v_st * 2) + vp[j];
+            kof[j] = row * (int)(a.k_st * 2) + (pk * 8 < a.dim ? pk * 16 : 0);
+            vof[j] = row * (int)(a.v_st * 2) + (pv * 8 < a.dim ? pv * 16 : 0);
         }
     }
     // Rows j0 .. of K and V to LDS; rows behind the last key repeat it, so what stands there is never read.
@@ -498,16 +514,12 @@ struct TileLoad {
         const char* kb = uniform_ptr(k + j0 * a.k_st);
         const char* vb = uniform_ptr(v + j0 * a.v_st);
         const bool whole = j0 + KT <= lk;
+        const int behind = row0 - (lk - 1 - j0);  // rows from the last key to row0
+        auto back = [&](int j) __attribute__((always_inline)) { return behind + j * RPI > 0 ? behind + j * RPI : 0; };
 #pragma unroll
-        for (int j = 0; j < NI; ++j) {
-            const int use = lk - 1 - j0;
-            glds16_asm(kb, whole ? kof[j] : (row[j] < use ? row[j] : use) * (int)(a.k_st * 2) + kp[j], kl + (wave * NI + j) * 1024);
-        }
+        for (int j = 0; j < NI; ++j) glds16_asm(kb, whole ? kof[j] : kof[j] - back(j) * (int)(a.k_st * 2), kl + (wave * NI + j) * 1024);
 #pragma unroll
-        for (int j = 0; j < NI; ++j) {
-            const int use = lk - 1 - j0;
-            glds16_asm(vb, whole ? vof[j] : (row[j] < use ? row[j] : use) * (int)(a.v_st * 2) + vp[j], vl + (wave * NI + j) * 1024);
-        }
+        for (int j = 0; j < NI; ++j) glds16_asm(vb, whole ? vof[j] : vof[j] - back(j) * (int)(a.v_st * 2), vl + (wave * NI + j) * 1024);
     }
 };
 
@@ -586,8 +598,8 @@ __device__ __forceinline__ float inverse(float l) { return l > 0.f || l != l ? 1
 // 1190, and what one side saves the clock (1.9 GHz under this load) or the other side eats.  Built and not kept, all
 // within 3 %: 64 rows per wave (half the LDS reads, two independent softmax chains), four waves per SIMD, three tiles in
 // flight, independent chains for maximum and sum.
-template <typename T, int DP, int BIAS, bool CAP, bool FIXED>
-__global__ __launch_bounds__(256, DP <= 64 && !(BIAS == BIAS_SLOPE && !CAP) ? 3 : DP <= 128 ? 2 : 1) void k_attend_rows(AttnArgs a) {
+template <typename T, int DP, int BIAS, int CAP, bool FIXED>
+__global__ __launch_bounds__(256, DP <= 64 && !(BIAS == BIAS_SLOPE && !CAP) && CAP != CAP_ANY ? 3 : DP <= 128 ? 2 : 1) void k_attend_rows(AttnArgs a) {
     constexpr int NB = DP <= 128 ? 2 : 1, KT = NB * 32, TILE = KT * DP * 2;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const float* table = (const float*)(lds + 4 * TILE);
@@ -653,7 +665,7 @@ __global__ __launch_bounds__(256, DP <= 64 && !(BIAS == BIAS_SLOPE && !CAP) ? 3 
 // ring of its own, without a barrier, and the waves' sums meet at the end in a fixed order.
 // Bound by HBM: 8 documents of 32768 keys, 8 key heads of 128, 4 query heads each: 214 us, 5.0 TB/s, the rate of a copy;
 // lengths of 1 .. 32768 171 us (4.3 TB/s; the longest document's chunks end last), with a cap and a slope 204 us.
-template <typename T, int DP, int NW, int BIAS, bool CAP, bool FIXED>
+template <typename T, int DP, int NW, int BIAS, int CAP, bool FIXED>
 __global__ __launch_bounds__(64 * NW) void k_attend_few(AttnArgs a) {
     constexpr int KT = 32, TILE = KT * DP * 2, ND = DP / 32, RING = 4 * TILE;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -808,7 +820,7 @@ static int launch_attend(hrs_ctx* ctx, hrs_per_device_once& attr, K kernel, int 
     HRS_CHECK_HIP(hipGetLastError());
     return HRS_OK;
 }
-template <typename T, int DP, int BIAS, bool CAP, bool FIXED>
+template <typename T, int DP, int BIAS, int CAP, bool FIXED>
 static int launch_fast(hrs_ctx* ctx, const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
     static hrs_per_device_once once_few, once_rows;
     const int table = BIAS == BIAS_TABLE ? a.group * (2 * (a.reach + TABLE_EDGE) + 1) * 4 : 0;
@@ -829,9 +841,10 @@ static int launch_form(hrs_ctx* ctx, const AttnArgs& a, const AttnPlan& p, hipSt
     // Capped scores without a bias lie within +-cap: in bf16, whose range is that of fp32, the weights need no running
     // maximum (2^+-80, their sum over 2^30 keys and its product with v stay inside fp32).
     if constexpr (CAP && BIAS == BIAS_NONE && __is_same(T, __bf16)) {
-        if (a.cap2 <= 80.f) return launch_fast<T, DP, BIAS, CAP, true>(ctx, a, p, st);
+        if (a.cap2 <= 80.f) return launch_fast<T, DP, BIAS, CAP_TO_64, true>(ctx, a, p, st);
     }
-    return launch_fast<T, DP, BIAS, CAP, false>(ctx, a, p, st);
+    if (CAP && a.cap2 > CAP_DIRECT) return launch_fast<T, DP, BIAS, CAP ? CAP_ANY : CAP_NONE, false>(ctx, a, p, st);
+    return launch_fast<T, DP, BIAS, CAP ? CAP_TO_64 : CAP_NONE, false>(ctx, a, p, st);
 }
 template <typename T, int DP>
 static int launch_dim(hrs_ctx* ctx, const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
@@ -909,6 +922,7 @@ static int attention_args(const hrs_attention_args* p, AttnArgs& a) {
     if (p->softcap > 0.f) {
         a.cap2 = p->softcap * LOG2E;
         a.cap_in = 2.f * LOG2E * p->scale / p->softcap;
+        a.cap_u = p->scale / p->softcap;
     }
     HRS_REQUIRE(a.scale2 < 1e30f && a.cap2 < 1e30f && a.cap_in < 1e30f, "hrs_attention: scale=%g with softcap=%g leaves the range of fp32", (double)p->scale, (double)p->softcap);
     return HRS_OK;

@@ -106,7 +106,9 @@ def attention(q, k, v, lq, lk, causal=False, prefix=None, scale=None, cap=0.0, s
         ds = 2 * (dim + 4) * F * scale * (qh.abs() @ kh.abs().t())
         if cap:
             s = cap * torch.tanh(s / cap)
-            ds = ds + 8 * F * cap  # cap - 2 cap / (1 + e): exp2, 1 / x and two roundings, all of size cap
+            # cap - 2 cap / (1 + e): exp2, 1 / x and two roundings, all of size cap; beyond 64 only where |s| > 0.38 cap, and
+            # tanh's series below (a dozen roundings of the result's size): relative to the score
+            ds = ds + (8 * F * cap if cap <= 64 else 24 * F * s.abs())
         x = s
         if slopes is not None:
             x = x - slopes[h].double() * dist.abs()
