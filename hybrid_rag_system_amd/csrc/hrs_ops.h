@@ -78,14 +78,14 @@ __device__ __forceinline__ float rcp_hw(float x) { return __builtin_amdgcn_rcpf(
 // (2.9e-5; the result is within 3.4e-5 of its own size on both sides of zero, a fifteenth of an fp16 half-step).  Two
 // transcendental and ten ordinary operations.
 __device__ __forceinline__ float gelu_f(float x) {
-    const float a = fabsf(x);
+    const float a = fabsf(fminf(x, 20.f));  // (e is 0 from 20 on, and 0 * inf would be NaN where x is inf)
     const float t = rcp_hw(fmaf(0.375f, a, 1.f));
     float q = fmaf(-0.0909841f, t, 0.20104071f);
     q = fmaf(q, t, 0.08297601f);
     q = fmaf(q, t, 0.15791951f);
     q = fmaf(q, t, 0.14904118f);
     const float e = exp2_hw(x * x * -0.72134752f);
-    return fmaxf(x, 0.f) - a * (t * q * e);
+    return fmaf(-a, t * q * e, fmaxf(x, 0.f));
 }
 __device__ __forceinline__ float sigmoid_f(float x) { return rcp_hw(1.f + exp2_hw(x * -1.44269504f)); }
 // tanh = 1 - 2 / (1 + e^2x) loses its leading digits near zero, where three terms of the series are exact to 2e-7

@@ -14,6 +14,25 @@ def _unaligned(t):
     return torch.cat([t, t[..., :1]], -1)[..., : t.shape[-1]]
 
 
+# ---- activations -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "gelu_tanh", "silu", "tanh"])
+@pytest.mark.parametrize("m,k", [(3, 64), (40, 64), (40, 63), (700, 64)])
+def test_linear_activations_of_infinities(eng, act, m, k):
+    """A sum of +-inf goes through every activation as its definition says (gelu, its tanh form and silu have 0 * inf below
+    zero), in every kernel; NaN stays NaN; large finite sums stay themselves or go to zero."""
+    inf, nan = float("inf"), float("nan")
+    b = torch.tensor([inf, -inf, nan, 3e4, -3e4, 1e38, -1e38, 0.0] * 32)
+    x, w = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda"), torch.zeros(256, k, dtype=torch.bfloat16, device="cuda")
+    got = eng.linear(x, w, b.cuda(), activation=act).cpu().float()
+    want = torch.tensor([inf, -inf, nan, 3e4, -3e4, 1e38, -1e38, 0.0]).double()
+    if act in ("none", "relu", "tanh"):
+        want = LO.activate(want, act)
+    else:
+        want[1], want[4], want[6] = nan, 0.0, 0.0
+    want = want.float().bfloat16().float()
+    assert torch.equal(torch.nan_to_num(got, nan=77.0), torch.nan_to_num(want, nan=77.0).repeat(32).expand(m, -1)), got[0, :8]
+
+
 # ---- score caps --------------------------------------------------------------------------------------
 @pytest.mark.parametrize("t", ["bf16", "fp16"])
 @pytest.mark.parametrize("cap", [66.0, 100.0, 1e3, 1e4, 1e6, 1e9, 1e29])
