@@ -104,6 +104,13 @@ __device__ __forceinline__ float capped(const AttnArgs& a, float s) {
     return t < 0.16f ? s * a.scale2 * p : capped_direct(a, s);
 }
 
+// A table's entry in base 2.  A finite one stays finite, also the type's lowest and largest values (log2 e times them would
+// be infinite): beyond +-1e30 entries count as they are.  NaN stays NaN.
+__device__ __forceinline__ float table2(float t) {
+    const float x = t * LOG2E;
+    return fabsf(x) < 1e30f || t != t ? x : t < 0.f ? fminf(t, -1e30f) : fmaxf(t, 1e30f);
+}
+
 // Score of one (query, key) pair in base 2: s is q . k, d = j - p_i.
 template <int BIAS, bool CAP>
 __device__ __forceinline__ float score2(const AttnArgs& a, float s, float slope2, const float* table, int d) {
@@ -111,9 +118,7 @@ __device__ __forceinline__ float score2(const AttnArgs& a, float s, float slope2
     if constexpr (BIAS == BIAS_SLOPE) x = fmaf(-slope2, fabsf((float)d), x);
     if constexpr (BIAS == BIAS_TABLE) {
         const int at = d < -a.reach ? -a.reach : d > a.reach ? a.reach : d;
-        const float t = table[at];
-        // a finite entry stays finite, also the type's lowest value (log2 e times it would be -inf)
-        x += fmaxf(t * LOG2E, fminf(t, -1e30f));
+        x += table2(table[at]);
     }
     return x;
 }
@@ -523,16 +528,14 @@ struct TileLoad {
     }
 };
 
-// Table rows of a key head's group, in base 2 (a finite entry stays finite, also the type's lowest value), each with its
-// first and last entry repeated TABLE_EDGE times.
+// Table rows of a key head's group, in base 2, each with its first and last entry repeated TABLE_EDGE times.
 __device__ __forceinline__ void stage_table(const AttnArgs& a, int hk, float* dst) {
     const int width = 2 * a.reach + 1, wide = width + 2 * TABLE_EDGE;
     for (int g = 0; g < a.group; ++g) {
         const float* src = a.table + (int64_t)(hk * a.group + g) * width;
         for (int i = threadIdx.x; i < wide; i += blockDim.x) {
             const int at = i - TABLE_EDGE;
-            const float t = src[at < 0 ? 0 : at < width ? at : width - 1];
-            dst[g * wide + i] = fmaxf(t * LOG2E, fminf(t, -1e30f));
+            dst[g * wide + i] = table2(src[at < 0 ? 0 : at < width ? at : width - 1]);
         }
     }
 }

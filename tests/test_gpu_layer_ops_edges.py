@@ -48,3 +48,29 @@ def test_attention_large_caps(eng, t, cap):
     got = eng.attention(*(_unaligned(x.cuda())[None] for x in (q, k, v)), softcap=cap)
     want, bound = LO.attention(q, k, v, 90, 90, cap=cap, dtype=TYPES[t])
     _close(got[0], want, bound)
+
+
+# ---- infinities and NaN in a bias table ----------------------------------------------------------------
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("queries,aligned", [(200, True), (2, True), (200, False)])
+def test_attention_table_with_nan_and_the_largest_value(eng, cap, queries, aligned):
+    """NaN at one distance reaches every query that sees a key there and no other; at the table's end it stands for all
+    distances beyond.  The type's largest value gives its key the whole weight."""
+    rnd, nan, keys = _gen(3), float("nan"), 300
+    q, k, v = rnd(1, queries, 2, 64).bfloat16(), rnd(1, keys, 2, 64).bfloat16(), rnd(1, keys, 2, 64).bfloat16()
+    dq, dk, dv = q.cuda(), k.cuda() if aligned else _unaligned(k.cuda()), v.cuda()
+    pos = torch.arange(queries) + keys - queries
+    for at, value in ((-20, nan), (5, nan), (-21, nan), (21, nan), (-3, torch.finfo(torch.float32).max), (-21, float("-inf")), (0, float("-inf"))):
+        table = rnd(2, 43) * 0.1
+        table[1, at + 21] = value
+        got = eng.attention(dq, dk, dv, causal=True, softcap=cap, bias_table=table.cuda())[0].cpu()
+        want, bound = LO.attention(q[0], k[0], v[0], queries, keys, causal=True, cap=cap, table=torch.nan_to_num(table, nan=0.0), dtype=torch.bfloat16)
+        if value != value:
+            hit = pos + at >= 0 if at <= 0 else torch.zeros(queries, dtype=torch.bool)  # (keys behind are not seen)
+            assert torch.isnan(got[:, 1]).all(-1).equal(hit) and torch.isnan(got[:, 1]).any(-1).equal(hit), at
+            got[hit, 1], want[hit, 1] = 0.0, 0.0
+        elif value > 0:
+            has = pos + at >= 0
+            assert torch.equal(got[has, 1], v[0, (pos + at)[has], 1])
+            got[has, 1], want[has, 1] = 0.0, 0.0
+        _close(got, want, bound + 1e-30, at)
