@@ -179,8 +179,8 @@ __global__ __launch_bounds__(256) void k_attend_any(AttnArgs a) {
             __syncthreads();
             for (int id2 = tid; id2 < KT * PPR; id2 += 256) {
                 const int i = id2 / PPR, p = id2 % PPR;
-                const int64_t j = j0 + i < dr.lk ? j0 + i : dr.lk - 1;  // what stands behind the document is never read
-                const int left = a.dim - p * 8;
+                const int64_t j = j0 + i;
+                const int left = j < dr.lk ? a.dim - p * 8 : 0;  // what stands behind the document is never read: zeros
                 *(x8*)(kl + i * (DP * 2) + place_k<DP>(i, p) * 16) = load8_any<T>(kbase + j * a.k_st + p * 8, left);
                 *(x8*)(vl + i * (DP * 2) + place_v<DP>(i, p) * 16) = load8_any<T>(vbase + j * a.v_st + p * 8, left);
             }
@@ -513,6 +513,11 @@ struct TileLoad {
             vof[j] = row * (int)(a.v_st * 2) + (pv * 8 < a.dim ? pv * 16 : 0);
         }
     }
+    // The wave's rows of V behind the last key, once they have landed: zero (0 times a V that is infinite there would be NaN).
+    __device__ __forceinline__ void blank_behind(int j0, int lk, uint32_t vl, int wave) const {
+        const int first = lk - j0 > wave * NI * RPI ? lk - j0 : wave * NI * RPI;
+        for (uint32_t at = vl + first * (DP * 2) + (threadIdx.x & 63) * 16; at < vl + (wave + 1) * NI * 1024; at += 1024) *(__attribute__((address_space(3))) u32x4*)(uintptr_t)at = (u32x4)(0u);
+    }
     // Rows j0 .. of K and V to LDS; rows behind the last key repeat it, so what stands there is never read.
     template <typename T>
     __device__ __forceinline__ void issue(const AttnArgs& a, const T* k, const T* v, int j0, int lk, uint32_t kl, uint32_t vl, int wave) {
@@ -645,6 +650,10 @@ __global__ __launch_bounds__(256, DP <= 64 && !(BIAS == BIAS_SLOPE && !CAP) && C
         st.open(a, dr, b, hk, prefix, row0 + wv * 32, r, table);
         int buf = 0;
         for (int j0 = from; j0 < need; j0 += KT, buf ^= 1) {
+            if (j0 + KT > dr.lk) {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                load.blank_behind(j0, dr.lk, l0 + buf * 2 * TILE + TILE, wv);
+            }
             wait_all_barrier();  // the tile has landed; everyone has read the one before
             if (j0 + KT < need) load.issue(a, kbase, vbase, j0 + KT, dr.lk, l0 + (buf ^ 1) * 2 * TILE, l0 + (buf ^ 1) * 2 * TILE + TILE, wv);
             if (j0 < st.lim_max) st.tile(a, lds + buf * 2 * TILE, lds + buf * 2 * TILE + TILE, table, j0);
@@ -711,6 +720,10 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(AttnArgs a) {
                 asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * TileLoad<DP, KT, 1>::NI) : "memory");
             } else {
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
+            if (j0 + KT > dr.lk) {
+                load.blank_behind(j0, dr.lk, l0 + buf * 2 * TILE + TILE, 0);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             }
             st.tile(a, mine + buf * 2 * TILE, mine + buf * 2 * TILE + TILE, table, j0);
         }

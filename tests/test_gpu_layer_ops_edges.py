@@ -74,3 +74,24 @@ def test_attention_table_with_nan_and_the_largest_value(eng, cap, queries, align
             assert torch.equal(got[has, 1], v[0, (pos + at)[has], 1])
             got[has, 1], want[has, 1] = 0.0, 0.0
         _close(got, want, bound + 1e-30, at)
+
+
+# ---- infinities in keys and values that every query sees -------------------------------------------------
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+@pytest.mark.parametrize("queries,aligned", [(70, True), (1, True), (70, False)])
+@pytest.mark.parametrize("dim", [64, 80])
+def test_attention_infinite_value_of_the_last_key(eng, queries, aligned, dim, t):
+    """A weight above zero times inf is inf, in that column alone, whether the last key ends a tile or not."""
+    for keys in (1, 33, 64, 65, 70, 127, 2000):
+        rnd = _gen(keys)
+        q, k, v = ((rnd(1, n, 2, dim) * 0.5).to(TYPES[t]) for n in (queries, keys, keys))
+        dq, dk, dv = q.cuda(), k.cuda(), v.cuda()
+        dv[0, -1, 1, 3] = float("inf")
+        if not aligned:
+            dk, dv = _unaligned(dk), _unaligned(dv)
+        got = eng.attention(dq, dk, dv)[0].cpu()
+        assert (got[:, 1, 3] == float("inf")).all(), keys
+        got[:, 1, 3] = 0
+        want, bound = LO.attention(q[0], k[0], v[0], queries, keys, dtype=TYPES[t])
+        want[:, 1, 3] = 0
+        _close(got, want, bound, keys)
