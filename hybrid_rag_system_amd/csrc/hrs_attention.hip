@@ -497,21 +497,48 @@ struct Attend {
     }
 };
 
+// glds16_asm for the lanes of `mask` alone.
+__device__ __forceinline__ void glds16_masked_asm(const void* sbase, int voff, uint32_t lds_addr, uint64_t mask) {
+    unsigned keep;
+    uint64_t lanes;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b64 %1, exec\n\ts_mov_b32 m0, %4\n\ts_and_b64 exec, exec, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b64 exec, %1\n\ts_mov_b32 m0, %0"
+        : "=&s"(keep), "=&s"(lanes)
+        : "v"(voff), "s"(sbase), "s"(lds_addr), "s"(mask)
+        : "memory", "scc");
+}
+
 // The wave's share of the DMA of one tile: KT rows of K and of V, NI instructions of 1 KB each.
 template <int DP, int KT, int NWAVES>
 struct TileLoad {
     static constexpr int PPR = DP / 8, RPI = 64 / PPR, NI = KT / RPI / NWAVES;
     int kof[NI], vof[NI], row0;  // this lane's row of instruction j is row0 + j RPI
+    // lanes whose piece of K is inside the head's dimension, for instruction j % NM (the swizzle repeats every 8 rows)
+    static constexpr int NM = RPI >= 8 ? 1 : 8 / RPI < NI ? 8 / RPI : NI;
+    uint64_t in_head[NM];
     __device__ __forceinline__ void open(const AttnArgs& a, int wave) {
         const int lane = threadIdx.x & 63;
         row0 = wave * NI * RPI + lane / PPR;
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
             const int row = row0 + j * RPI, pk = (lane % PPR) ^ swizzle_k<DP>(row), pv = (lane % PPR) ^ swizzle_v<DP>(row);
-            // (a piece behind the head's dimension repeats the first: it meets zeros of q, or ends in columns not stored)
-            kof[j] = row * (int)(a.k_st * 2) + (pk * 8 < a.dim ? pk * 16 : 0);
+            // (a piece of V behind the head's dimension repeats the first: it ends in columns not stored)
+            kof[j] = row * (int)(a.k_st * 2) + pk * 16;
+            if (j < NM) in_head[j] = __ballot(pk * 8 < a.dim);
             vof[j] = row * (int)(a.v_st * 2) + (pv * 8 < a.dim ? pv * 16 : 0);
         }
+    }
+    // Pieces of K behind the head's dimension are never fetched and meet zeros of q: zero in both buffers (0 times whatever
+    // stood there could be NaN).
+    __device__ __forceinline__ void blank_pads(const AttnArgs& a, uint32_t kl, int next, int wave) const {
+        if (a.dim == DP) return;
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+            if (!(in_head[j % NM] >> (threadIdx.x & 63) & 1)) {
+                const uint32_t at = kl + (wave * NI + j) * 1024 + (threadIdx.x & 63) * 16;
+                *(__attribute__((address_space(3))) u32x4*)(uintptr_t)at = (u32x4)(0u);
+                *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(at + next) = (u32x4)(0u);
+            }
     }
     // The wave's rows of V behind the last key, once they have landed: zero (0 times a V that is infinite there would be NaN).
     __device__ __forceinline__ void blank_behind(int j0, int lk, uint32_t vl, int wave) const {
@@ -526,8 +553,13 @@ struct TileLoad {
         const bool whole = j0 + KT <= lk;
         const int behind = row0 - (lk - 1 - j0);  // rows from the last key to row0
         auto back = [&](int j) __attribute__((always_inline)) { return behind + j * RPI > 0 ? behind + j * RPI : 0; };
+        if (a.dim == DP) {
 #pragma unroll
-        for (int j = 0; j < NI; ++j) glds16_asm(kb, whole ? kof[j] : kof[j] - back(j) * (int)(a.k_st * 2), kl + (wave * NI + j) * 1024);
+            for (int j = 0; j < NI; ++j) glds16_asm(kb, whole ? kof[j] : kof[j] - back(j) * (int)(a.k_st * 2), kl + (wave * NI + j) * 1024);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NI; ++j) glds16_masked_asm(kb, whole ? kof[j] : kof[j] - back(j) * (int)(a.k_st * 2), kl + (wave * NI + j) * 1024, in_head[j % NM]);
+        }
 #pragma unroll
         for (int j = 0; j < NI; ++j) glds16_asm(vb, whole ? vof[j] : vof[j] - back(j) * (int)(a.v_st * 2), vl + (wave * NI + j) * 1024);
     }
@@ -628,6 +660,7 @@ __global__ __launch_bounds__(256, DP <= 64 && !(BIAS == BIAS_SLOPE && !CAP) && C
     TileLoad<DP, KT, 4> load;
     load.open(a, wv);
     const uint32_t l0 = lds_addr_of(lds);
+    load.blank_pads(a, l0, 2 * TILE, wv);
     // keys that any of the workgroup's rows from row0 on sees, in this chunk; the first tile of them is requested at once
     auto begin = [&](int row0) __attribute__((always_inline)) {
         if (row0 >= rows) return 0;
@@ -711,6 +744,7 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(AttnArgs a) {
         if (need > from + a.chunk) need = from + a.chunk;
         int buf = 0;
         const int first = from + wv * KT;
+        load.blank_pads(a, l0, 2 * TILE, 0);
         if (first < need) load.issue(a, kbase, vbase, first, dr.lk, l0, l0 + TILE, 0);
         for (int j0 = first; j0 < need; j0 += NW * KT, buf ^= 1) {
             // this wave's reads of the other buffer are done (the products that needed them are under way)

@@ -95,3 +95,22 @@ def test_attention_infinite_value_of_the_last_key(eng, queries, aligned, dim, t)
         want, bound = LO.attention(q[0], k[0], v[0], queries, keys, dtype=TYPES[t])
         want[:, 1, 3] = 0
         _close(got, want, bound, keys)
+
+
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+@pytest.mark.parametrize("queries,heads,aligned", [(70, 2, True), (1, 2, True), (70, 2, False), (20, 6, True)])
+@pytest.mark.parametrize("dim", [8, 16, 40, 64, 80, 120, 136, 256])
+def test_attention_infinite_key_has_no_weight(eng, queries, heads, aligned, dim, t):
+    """A key whose products with every query are -inf weighs nothing, at every head width: as if it were not there."""
+    rnd = _gen(dim)
+    for keys, gone in ((90, 3), (70, 69), (1500, 777)):
+        q, k, v = ((rnd(1, n, h, dim) * 0.5).to(TYPES[t]) for n, h in ((queries, heads), (keys, 2), (keys, 2)))
+        q = q.abs() + 0.25
+        dq, dk, dv = q.cuda(), k.cuda(), v.cuda()
+        dk[0, gone, :, 0] = dk[0, gone, :, dim - 1] = dk[0, gone, :, dim // 2] = -float("inf")
+        if not aligned:
+            dk, dv = _unaligned(dk), _unaligned(dv)
+        got = eng.attention(dq, dk, dv)[0].cpu()
+        rest = [j for j in range(keys) if j != gone]
+        want, bound = LO.attention(q[0], k[0, rest], v[0, rest], queries, keys - 1, dtype=TYPES[t])
+        _close(got, want, bound, (keys, gone))
