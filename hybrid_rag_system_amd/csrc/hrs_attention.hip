@@ -216,9 +216,9 @@ __global__ __launch_bounds__(256) void k_attend_any(AttnArgs a) {
             for (int n = 0; n < NB; ++n)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const float w = exp2_hw(s[n][r] - base);
-                    l += w;
-                    pf[2 * n + (r >> 3)][r & 7] = (T)w;
+                    const T w = (T)exp2_hw(s[n][r] - base);
+                    l += (float)w;  // (the rounded weight: numerator and denominator round alike)
+                    pf[2 * n + (r >> 3)][r & 7] = w;
                 }
             // step t: keys 16 t + 8 e + 4 h + (0 .. 3) of the tile, e = 0, 1
 #pragma unroll

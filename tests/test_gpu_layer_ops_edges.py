@@ -1,5 +1,7 @@
 """hrs_linear, hrs_attention and hrs_layer_norm at the ends of what their documentation allows: score caps of any size,
 infinities and NaN, weights far below a row's largest, very wide outputs.  Definitions and bounds: oracle/layer_oracle.py."""
+import math
+
 import pytest
 import torch
 
@@ -114,3 +116,21 @@ def test_attention_infinite_key_has_no_weight(eng, queries, heads, aligned, dim,
         rest = [j for j in range(keys) if j != gone]
         want, bound = LO.attention(q[0], k[0, rest], v[0, rest], queries, keys - 1, dtype=TYPES[t])
         _close(got, want, bound, (keys, gone))
+
+
+# ---- weights -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+@pytest.mark.parametrize("queries,aligned", [(70, True), (1, True), (70, False), (1, False)])
+def test_attention_of_one_value_is_that_value(eng, queries, aligned, t):
+    """All values alike: the weights' rounding cancels between numerator and denominator, in every kernel.  All but one of
+    the weights stand just above the middle of two numbers of the type, the value just below a power of two."""
+    step = torch.finfo(TYPES[t]).eps / 2  # of the numbers in [0.5, 1)
+    weight, value = 0.5 + 0.55 * step, 2 - 2 * step
+    q, k = torch.zeros(1, queries, 1, 64), torch.zeros(1, 101, 1, 64)
+    q[..., 0], k[:, 1:, :, 0] = 1, -1
+    v = torch.full((1, 101, 1, 64), value)
+    q, k, v = (x.to(TYPES[t]).cuda() for x in (q, k, v))
+    if not aligned:
+        k, v = _unaligned(k), _unaligned(v)
+    got = eng.attention(q, k, v, scale=-math.log(weight))
+    assert (got == value).all(), got[0, 0, 0, 0].item()
