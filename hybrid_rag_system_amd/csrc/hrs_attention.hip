@@ -111,6 +111,11 @@ __device__ __forceinline__ float table2(float t) {
     return fabsf(x) < 1e30f || t != t ? x : t < 0.f ? fminf(t, -1e30f) : fmaxf(t, 1e30f);
 }
 
+// Weights are 2^(x - base) up to a factor that cancels in the quotient.  In fp16, where 2^-25 rounds to nothing, the largest
+// is put near the top of its range instead of at 1, or many keys of 2^-26 each would be mass lost (1.6 % for a million of them).
+template <typename T>
+constexpr float top_weight(float largest) { return __is_same(T, _Float16) ? 15.f - largest : 0.f; }
+
 // Score of one (query, key) pair in base 2: s is q . k, d = j - p_i.
 template <int BIAS, bool CAP>
 __device__ __forceinline__ float score2(const AttnArgs& a, float s, float slope2, const float* table, int d) {
@@ -205,21 +210,22 @@ __global__ __launch_bounds__(256) void k_attend_any(AttnArgs a) {
                 }
             top = fmaxf(top, swap_halves(top));
             const float m_new = fmaxf(m, top);
-            const float base = m_new == -INFINITY ? 0.f : m_new;  // nothing seen so far: every weight is exp2(-inf) = 0
-            const float keep = exp2_hw(m - base);
+            const float keep = exp2_hw(m - (m_new == -INFINITY ? 0.f : m_new));
+            const float base = m_new == -INFINITY ? 0.f : m_new - top_weight<T>(0.f);  // nothing seen so far: every weight is exp2(-inf) = 0
             m = m_new;
-            l *= keep;
 #pragma unroll
             for (int i = 0; i < ND; ++i) acc[i] *= keep;
             x8 pf[2 * NB];
+            float part = 0.f;  // (a tile's weights are summed before they meet the running sum, beside which single ones may be nothing)
 #pragma unroll
             for (int n = 0; n < NB; ++n)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const T w = (T)exp2_hw(s[n][r] - base);
-                    l += (float)w;  // (the rounded weight: numerator and denominator round alike)
+                    part += (float)w;  // (the rounded weight: numerator and denominator round alike)
                     pf[2 * n + (r >> 3)][r & 7] = w;
                 }
+            l = fmaf(l, keep, part);
             // step t: keys 16 t + 8 e + 4 h + (0 .. 3) of the tile, e = 0, 1
 #pragma unroll
             for (int t = 0; t < 2 * NB; ++t)
@@ -449,8 +455,8 @@ struct Attend {
                 top = fmaxf(top, fmaf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), mul, off[n]));
             }
             top = fmaxf(top, swap_halves(top));
-            // The base m of a row's weights follows its maximum only when that is 2^8 ahead: weights up to 256 are as exact
-            // as those up to 1 (fp16's largest is 65504), and the sums need not be rescaled each time some row of the
+            // The base m of a row's weights follows its maximum only when that is 2^8 ahead: weights up to 2^8 (in fp16 from
+            // 2^7 to 2^15; its largest is 65504) are as exact as those up to 1, and the sums need not be rescaled each time some row of the
             // wave finds a new maximum, which over 8192 keys of random scores is in three tiles of five.
             if (__any(top > m + 8.f)) {
                 const float m_new = fmaxf(m, top);
@@ -460,13 +466,14 @@ struct Attend {
 #pragma unroll
                 for (int i = 0; i < ND; ++i) acc[i] *= keep;
             }
-            const float base = m == -INFINITY ? 0.f : m;  // nothing seen so far: every weight is exp2(-inf) = 0
+            const float base = m == -INFINITY ? 0.f : m - top_weight<T>(8.f);  // nothing seen so far: every weight is exp2(-inf) = 0
 #pragma unroll
             for (int n = 0; n < NB; ++n) off[n] -= base;
         }
-        // The sum of weights is that of the rounded ones, two per instruction: numerator and denominator round alike.
+        // The sum of weights is that of the rounded ones, two per instruction: numerator and denominator round alike.  A tile's
+        // are summed before they meet the running sum, beside which single ones may be nothing.
         x8 pf[2 * NB];
-        float part[4] = {l, 0.f, 0.f, 0.f};
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -478,7 +485,7 @@ struct Attend {
                 pf[2 * n + (e >> 3)][e & 7] = w[0];
                 pf[2 * n + (e >> 3)][(e & 7) + 1] = w[1];
             }
-        l = (part[0] + part[1]) + (part[2] + part[3]);
+        l += (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
         for (int t = 0; t < 2 * NB; ++t)
 #pragma unroll

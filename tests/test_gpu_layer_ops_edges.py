@@ -134,3 +134,22 @@ def test_attention_of_one_value_is_that_value(eng, queries, aligned, t):
         k, v = _unaligned(k), _unaligned(v)
     got = eng.attention(q, k, v, scale=-math.log(weight))
     assert (got == value).all(), got[0, 0, 0, 0].item()
+
+
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+@pytest.mark.parametrize("queries,heads,aligned", [(70, 520, True), (1, 520, True), (70, 1, True), (70, 1, False), (1, 1, False)])
+def test_attention_many_small_weights_are_not_lost(eng, queries, heads, aligned, t):
+    """One key of weight 1 and 2^17 of 2^-26 each, half of what rounds to nothing in fp16: together 2^-9, which moves the
+    result by 2^-8.  520 heads (of the same numbers): a row's keys are not cut into chunks, which have maxima of their own."""
+    n = 1 << 17
+    q, k, v = torch.zeros(1, queries, 1, 32), torch.zeros(1, n + 1, 1, 32), torch.full((1, n + 1, 1, 32), -1.0)
+    q[..., 0], k[:, 1:, :, 0], v[:, 0] = 1, -1, 1
+    q, k, v = (x.to(TYPES[t]).cuda() for x in (q, k, v))
+    if not aligned:
+        k, v = _unaligned(k), _unaligned(v)
+    got = eng.attention(*(x.expand(-1, -1, heads, -1) for x in (q, k, v)), scale=26 * math.log(2)).double()
+    mass = n * 2.0**-26
+    # The weights are exact but for the scale's rounding (2^-23 of an exponent of 26).  The running sum of weights takes a
+    # tile of 32 keys at least with one rounding of 2^-24, the products 16 keys with one of 2^-23 at most.
+    tol = LO.half_step(TYPES[t]) + (n / 32 + 2 * n / 16) * 2.0**-24 + 2 * mass * 2.0**-18
+    assert (got - (1 - mass) / (1 + mass)).abs().max() <= tol
