@@ -985,8 +985,9 @@ static int attention_args(const hrs_attention_args* p, AttnArgs& a) {
     return HRS_OK;
 }
 
-// How the work is cut, from the arguments alone (never from device data).
-static AttnPlan plan_attention(hrs_ctx* ctx, const hrs_attention_args* p, AttnArgs& a) {
+// How the work is cut, from the arguments alone (never from device data).  A call whose addresses are not 16-byte aligned
+// needs no workspace; the size of one is asked for as if they were.
+static AttnPlan plan_attention(hrs_ctx* ctx, const hrs_attention_args* p, AttnArgs& a, bool aligned) {
     AttnPlan plan;
     // without a hint for packed documents: twice their mean
     const int64_t mean_q = a.q_offs && a.batch ? (2 * a.q_rows + a.batch - 1) / a.batch : a.q_rows;
@@ -1001,9 +1002,8 @@ static AttnPlan plan_attention(hrs_ctx* ctx, const hrs_attention_args* p, AttnAr
     a.chunks = 1;
     a.chunk = 1 << 30;
     // 16-byte pieces, and 64 rows of K or V within the 2^31 bytes that a DMA's lane offset spans
-    const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out;
     const int64_t strides = a.q_sb | a.q_st | a.q_sh | a.k_sb | a.k_st | a.k_sh | a.v_sb | a.v_st | a.v_sh;
-    plan.fast = at % 16 == 0 && strides % 8 == 0 && a.k_st < (1 << 23) && a.v_st < (1 << 23) &&
+    plan.fast = aligned && strides % 8 == 0 && a.k_st < (1 << 23) && a.v_st < (1 << 23) &&
                 (!a.table || (int64_t)a.group * (2 * (a.reach + TABLE_EDGE) + 1) * 4 <= ATTN_TABLE_LDS);
     if (!plan.fast) return plan;
     plan.few = rows <= 32;
@@ -1046,14 +1046,9 @@ static AttnPlan plan_attention(hrs_ctx* ctx, const hrs_attention_args* p, AttnAr
     return plan;
 }
 
-static int check_attention(hrs_ctx* ctx, const hrs_attention_args* p, AttnArgs& a) {
-    int rc = attention_args(p, a);
-    if (rc) return rc;
-    if (a.batch == 0 || a.q_rows == 0) return HRS_OK;
+static bool nothing_to_do(const AttnArgs& a) { return a.batch == 0 || a.q_rows == 0; }
+static int operands_given(const AttnArgs& a) {
     HRS_REQUIRE(a.q && a.out && (a.k_rows == 0 || (a.k && a.v)), "hrs_attention: null operand");
-    HRS_REQUIRE(a.out != a.q && a.out != a.k && a.out != a.v, "hrs_attention: out may not be an input");
-    HRS_REQUIRE(((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out) % 2 == 0, "hrs_attention: an operand is not aligned to its elements");
-    (void)ctx;
     return HRS_OK;
 }
 
@@ -1061,18 +1056,21 @@ extern "C" int hrs_attention_workspace(hrs_ctx* ctx, const hrs_attention_args* p
     HRS_REQUIRE(ctx && p && bytes, "hrs_attention_workspace: null argument");
     *bytes = 0;
     AttnArgs a;
-    int rc = check_attention(ctx, p, a);
-    if (rc || a.batch == 0 || a.q_rows == 0) return rc;
-    *bytes = plan_attention(ctx, p, a).bytes;
+    int rc = attention_args(p, a);
+    if (rc || nothing_to_do(a) || (rc = operands_given(a))) return rc;
+    *bytes = plan_attention(ctx, p, a, true).bytes;
     return HRS_OK;
 }
 
 extern "C" int hrs_attention(hrs_ctx* ctx, const hrs_attention_args* p, void* stream) {
     HRS_REQUIRE(ctx && p, "hrs_attention: null argument");
     AttnArgs a;
-    int rc = check_attention(ctx, p, a);
-    if (rc || a.batch == 0 || a.q_rows == 0) return rc;
-    const AttnPlan plan = plan_attention(ctx, p, a);
+    int rc = attention_args(p, a);
+    if (rc || nothing_to_do(a) || (rc = operands_given(a))) return rc;
+    HRS_REQUIRE(a.out != a.q && a.out != a.k && a.out != a.v, "hrs_attention: out may not be an input");
+    const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out;
+    HRS_REQUIRE(at % 2 == 0, "hrs_attention: an operand is not aligned to its elements");
+    const AttnPlan plan = plan_attention(ctx, p, a, at % 16 == 0);
     if (plan.bytes) {
         HRS_REQUIRE(p->workspace && p->workspace_bytes >= plan.bytes && (uintptr_t)p->workspace % 16 == 0,
                     "hrs_attention: a workspace of %zu bytes (given: %zu), 16-byte aligned, is needed", plan.bytes, p->workspace ? p->workspace_bytes : (size_t)0);

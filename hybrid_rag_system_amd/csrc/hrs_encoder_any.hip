@@ -236,11 +236,7 @@ int hrs_encoder_any_run(hrs_ctx* ctx, hrs_encoder_any* e, const int32_t* ids_dev
     at.q_offs = at.k_offs = offs_dev;
     at.q_lens = at.k_lens = lens_dev;
     at.max_q = at.max_k = longest;
-    // (the plan of a call depends on the alignment of its pointers: the workspace's parts lie at multiples of 256 bytes)
-    at.q = (const void*)256;
-    at.k = (const char*)at.q + (size_t)H * 2;
-    at.v = (const char*)at.k + (size_t)H * 2;
-    at.out = (void*)((size_t)1 << 20);
+    at.q = at.k = at.v = at.out = out_dev;  // (asking for the workspace's size only takes them not to be null)
     size_t need = 0;
     int rc = hrs_attention_workspace(ctx, &at, &need);
     if (rc) return rc;

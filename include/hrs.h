@@ -264,8 +264,8 @@ typedef struct hrs_attention_args {
 /* A query that sees no key gets zeros.  Weights are rounded to dtype before they meet v; sums and statistics are fp32.
  * k and v must be finite inside a document where a query of the same 128 rows may not see them (0 * inf is NaN). */
 int hrs_attention(hrs_ctx* ctx, const hrs_attention_args* args, void* stream);
-/* Bytes of workspace hrs_attention needs for these arguments (0 for most); the pointers in args are not looked at beyond
- * being null or not. */
+/* Bytes of workspace hrs_attention needs for these arguments (0 for most).  Of the pointers in args only whether they are
+ * null counts: the answer is enough for any addresses. */
 int hrs_attention_workspace(hrs_ctx* ctx, const hrs_attention_args* args, size_t* bytes);
 
 /* y = (z - mean z) / sqrt(var z + eps) * gamma + beta with z = x + r, row by row: x, r (nullable) and y [M, N] of type
