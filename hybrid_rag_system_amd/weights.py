@@ -13,6 +13,7 @@ Linear weights are [out, in] (y = x @ w.T + b), as BERT stores them.
 """
 import json
 import os
+import warnings
 from dataclasses import dataclass
 
 import numpy as np
@@ -37,18 +38,44 @@ class EncoderConfig:
     @classmethod
     def from_dir(cls, path):
         """The geometry a local model directory names in its `config.json` (BERT's keys); without that file, or without a
-        key, the default's."""
+        key, the default's.  What the directory's sentence-transformers files say of pooling is checked (check_modules)."""
+        check_modules(path)
         file = os.path.join(path, "config.json")
-        if not os.path.exists(file):
-            return cls()
-        with open(file, encoding="utf-8") as f:
-            raw = json.load(f)
+        raw = read_json(path, "config.json")
         keys = {"vocab": "vocab_size", "hidden": "hidden_size", "layers": "num_hidden_layers", "heads": "num_attention_heads", "inter": "intermediate_size",
                 "max_pos": "max_position_embeddings", "eps": "layer_norm_eps"}
         for key, want in (("model_type", "bert"), ("hidden_act", "gelu"), ("position_embedding_type", "absolute")):
             if raw.get(key, want) != want:
                 raise ValueError(f"{file}: {key} {raw[key]!r} is not the encoder built here ({want})")
         return cls(**{ours: type(getattr(cls, ours))(raw[theirs]) for ours, theirs in keys.items() if theirs in raw})
+
+
+def read_json(path, *names):
+    """A directory's JSON file, {} where it has none."""
+    file = os.path.join(path, *names)
+    if not os.path.exists(file):
+        return {}
+    with open(file, encoding="utf-8") as f:
+        return json.load(f)
+
+
+def check_modules(path):
+    """What stands behind the transformer in a model directory (modules.json, the pooling's config.json): the encoder here
+    takes the mean over the tokens and gives rows of unit length.  Another pooling or another module is another embedding:
+    ValueError.  Without a Normalize module the model's own rows have other lengths (and the same directions): a warning."""
+    modules = read_json(path, "modules.json") or [{"type": "Transformer", "path": ""}, {"type": "Pooling", "path": "1_Pooling"}, {"type": "Normalize"}]
+    for m in modules:
+        kind = m["type"].split(".")[-1]
+        if kind not in ("Transformer", "Pooling", "Normalize"):
+            raise ValueError(f"{path}: module {m['type']} is not built here (a mean over tokens, of unit length, is)")
+        if kind == "Pooling":
+            raw = read_json(path, m["path"], "config.json")
+            modes = [k[len("pooling_mode_") :] for k, v in raw.items() if k.startswith("pooling_mode_") and v]
+            modes += [raw["pooling_mode"]] if "pooling_mode" in raw else []
+            if raw and modes not in (["mean_tokens"], ["mean"]):
+                raise ValueError(f"{os.path.join(path, m['path'])}: pooling by {' and '.join(modes) or 'nothing'} is not built here (the mean over tokens is)")
+    if not any(m["type"].split(".")[-1] == "Normalize" for m in modules):
+        warnings.warn(f"{path}: the model does not normalise its embeddings, the rows given here have unit length", stacklevel=3)
 
 
 def tensor_specs(cfg):

@@ -1,0 +1,51 @@
+"""What a local model directory says beside its geometry: pooling, modules, tokeniser (the files sentence-transformers writes
+next to a model; the reference names one at scripts/chromadb_helper.py:64-66).  Followed, or refused."""
+import json
+import warnings
+
+import pytest
+
+from hybrid_rag_system_amd import weights as W
+
+
+def _write(path, **files):
+    for name, content in files.items():
+        f = path / name
+        f.parent.mkdir(exist_ok=True)
+        f.write_text(json.dumps(content))
+
+
+def _pooling(**modes):
+    return {"word_embedding_dimension": 128, **{f"pooling_mode_{k}": False for k in ("cls_token", "mean_tokens", "max_tokens", "mean_sqrt_len_tokens")}, **{f"pooling_mode_{k}": v for k, v in modes.items()}}
+
+
+MODULES = [{"idx": 0, "name": "0", "path": "", "type": "sentence_transformers.models.Transformer"}, {"idx": 1, "name": "1", "path": "1_Pooling", "type": "sentence_transformers.models.Pooling"},
+           {"idx": 2, "name": "2", "path": "2_Normalize", "type": "sentence_transformers.models.Normalize"}]
+
+
+@pytest.mark.parametrize("modules", [None, MODULES, [MODULES[0], {**MODULES[1], "path": "other"}, MODULES[2]]])
+def test_pooling_is_the_mean_or_refused(tmp_path, modules):
+    if modules:
+        _write(tmp_path, **{"modules.json": modules})
+    where = modules[1]["path"] if modules else "1_Pooling"
+    assert W.EncoderConfig.from_dir(str(tmp_path)) == W.EncoderConfig()
+    for good in (_pooling(mean_tokens=True), {"pooling_mode": "mean"}):
+        _write(tmp_path, **{f"{where}/config.json": good})
+        assert W.EncoderConfig.from_dir(str(tmp_path)) == W.EncoderConfig()
+    for bad in (_pooling(cls_token=True), _pooling(max_tokens=True), _pooling(mean_tokens=True, cls_token=True), _pooling(mean_sqrt_len_tokens=True), _pooling(), _pooling(lasttoken=True), {"pooling_mode": "cls"}):
+        _write(tmp_path, **{f"{where}/config.json": bad})
+        with pytest.raises(ValueError, match="pooling"):
+            W.EncoderConfig.from_dir(str(tmp_path))
+
+
+def test_other_modules_are_refused_and_a_missing_norm_is_told(tmp_path):
+    _write(tmp_path, **{"modules.json": MODULES[:2] + [{"idx": 2, "name": "2", "path": "2_Dense", "type": "sentence_transformers.models.Dense"}]})
+    with pytest.raises(ValueError, match="Dense"):
+        W.EncoderConfig.from_dir(str(tmp_path))
+    _write(tmp_path, **{"modules.json": MODULES[:2]})
+    with pytest.warns(UserWarning, match="normalise"):
+        W.EncoderConfig.from_dir(str(tmp_path))
+    _write(tmp_path, **{"modules.json": MODULES})
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        W.EncoderConfig.from_dir(str(tmp_path))
