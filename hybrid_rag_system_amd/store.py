@@ -39,8 +39,9 @@ class HrsEmbeddingFunction:
     (scripts/chromadb_helper.py:64-66): tokenise on the host, encode on the GPU, unit-norm rows.
 
     model_dir (or $HRS_MODEL_DIR) may hold `vocab.txt` + `model.safetensors` of a MiniLM-L6 class
-    model, or of a BERT of another geometry with its `config.json`; without it the generated weights
-    and the hash tokeniser are used (no hub access exists).
+    model, or of a BERT of another geometry with its `config.json`; what its other files say of
+    pooling and of the tokeniser is followed or, where it is not built here, refused.  Without a
+    directory the generated weights and the hash tokeniser are used (no hub access exists).
     """
 
     def __init__(self, model_name="all-MiniLM-L6-v2", model_dir=None, seed=2026, batch_size=1024):
@@ -50,7 +51,7 @@ class HrsEmbeddingFunction:
         if model_dir and os.path.exists(os.path.join(model_dir, "model.safetensors")):
             self.cfg = W.EncoderConfig.from_dir(model_dir)
             weights = W.load_safetensors(model_dir, self.cfg)
-            self.tokenizer = WordPieceTokenizer(os.path.join(model_dir, "vocab.txt"))
+            self.tokenizer = WordPieceTokenizer.from_dir(model_dir)
             self.source = model_dir
         else:
             weights = W.generate(self.cfg, seed)

@@ -20,6 +20,8 @@ import unicodedata
 
 import numpy as np
 
+from .weights import read_json
+
 CLS_ID, SEP_ID, PAD_ID, UNK_ID = 101, 102, 0, 100  # the ids bert-base-uncased style vocabularies use
 
 
@@ -164,6 +166,19 @@ class WordPieceTokenizer(_Base):
         self.cls_id, self.sep_id = self.vocab["[CLS]"], self.vocab["[SEP]"]
         self.pad_id, self.unk_id = self.vocab.get("[PAD]", 0), self.vocab["[UNK]"]
         self._vocab_list = list(vocab)
+
+    @classmethod
+    def from_dir(cls, path):
+        """`vocab.txt` of a local model directory, cased or not as its `tokenizer_config.json` says (without it: not).
+        Another tokeniser than BERT's, or BERT's with other switches, is a ValueError."""
+        raw = read_json(path, "tokenizer_config.json")
+        lower = raw.get("do_lower_case", True)
+        for key, ours in (("tokenizer_class", ("BertTokenizer", "BertTokenizerFast")), ("strip_accents", (None, lower)), ("tokenize_chinese_chars", (True,)), ("do_basic_tokenize", (True,))):
+            if raw.get(key, ours[0]) not in ours:
+                raise ValueError(f"{os.path.join(path, 'tokenizer_config.json')}: {key} {raw[key]!r} is not the tokeniser built here ({ours[0]})")
+        if read_json(path, "sentence_bert_config.json").get("do_lower_case") and not lower:
+            raise ValueError(f"{path}: lower case in front of a cased tokeniser is not built here")
+        return cls(os.path.join(path, "vocab.txt"), lower=bool(lower))
 
     def _vocab_blob(self):
         return "\n".join(self._vocab_list).encode("utf-8", "surrogatepass")

@@ -6,6 +6,9 @@ import warnings
 import pytest
 
 from hybrid_rag_system_amd import weights as W
+from hybrid_rag_system_amd.tokenizer import WordPieceTokenizer
+
+VOCAB = ["[PAD]", "[UNK]", "[CLS]", "[SEP]", "server", "Server", "caf\u00e9", "cafe"]
 
 
 def _write(path, **files):
@@ -49,3 +52,22 @@ def test_other_modules_are_refused_and_a_missing_norm_is_told(tmp_path):
     with warnings.catch_warnings():
         warnings.simplefilter("error")
         W.EncoderConfig.from_dir(str(tmp_path))
+
+
+def test_tokeniser_is_cased_where_the_directory_says_so(tmp_path):
+    (tmp_path / "vocab.txt").write_text("\n".join(VOCAB) + "\n", encoding="utf-8")
+    text = "Server server caf\u00e9"
+    assert WordPieceTokenizer.from_dir(str(tmp_path)).encode(text) == [2, 4, 4, 7, 3]
+    for config, want in (({"do_lower_case": True, "tokenizer_class": "BertTokenizer", "strip_accents": None}, [2, 4, 4, 7, 3]), ({"do_lower_case": False, "tokenizer_class": "BertTokenizerFast"}, [2, 5, 4, 6, 3])):
+        _write(tmp_path, **{"tokenizer_config.json": config})
+        tok = WordPieceTokenizer.from_dir(str(tmp_path))
+        assert tok.encode(text) == want
+        ids, lens = tok.encode_batch([text])  # the native rules
+        assert ids[0, : lens[0]].tolist() == want
+    for bad in ({"do_lower_case": True, "strip_accents": False}, {"do_lower_case": False, "strip_accents": True}, {"tokenize_chinese_chars": False}, {"tokenizer_class": "MPNetTokenizer"}):
+        _write(tmp_path, **{"tokenizer_config.json": bad})
+        with pytest.raises(ValueError, match="not the tokeniser"):
+            WordPieceTokenizer.from_dir(str(tmp_path))
+    _write(tmp_path, **{"tokenizer_config.json": {"do_lower_case": False}, "sentence_bert_config.json": {"do_lower_case": True}})
+    with pytest.raises(ValueError, match="lower case"):
+        WordPieceTokenizer.from_dir(str(tmp_path))
