@@ -51,7 +51,7 @@ class HrsEmbeddingFunction:
         if model_dir and os.path.exists(os.path.join(model_dir, "model.safetensors")):
             self.cfg = W.EncoderConfig.from_dir(model_dir)
             weights = W.load_safetensors(model_dir, self.cfg)
-            self.tokenizer = WordPieceTokenizer.from_dir(model_dir)
+            self.tokenizer = WordPieceTokenizer.from_dir(model_dir, self.cfg.max_seq)
             self.source = model_dir
         else:
             weights = W.generate(self.cfg, seed)

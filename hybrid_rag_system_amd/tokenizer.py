@@ -88,7 +88,7 @@ class _Base:
         """-> (ids int32 [B, S] padded, lens int32 [B]); S = longest row rounded up to a multiple of 32."""
         rows = [self.encode(t) for t in texts]
         longest = max((len(r) for r in rows), default=2)
-        S = min(256, (longest + 31) // 32 * 32)
+        S = (longest + 31) // 32 * 32
         ids = np.full((len(rows), S), self.pad_id, np.int32)
         lens = np.zeros(len(rows), np.int32)
         for b, r in enumerate(rows):
@@ -121,13 +121,13 @@ class _Base:
 
         texts = list(texts)
         B = len(texts)
-        if B == 0 or self.max_len > 256:
+        if B == 0 or self.max_len > 512:  # (what hrs_tokenize takes)
             return self.encode_batch_python(texts)
         raw = [t.encode("utf-8", "surrogatepass") for t in texts]
         offs = np.zeros(B + 1, np.int64)
         np.cumsum([len(r) for r in raw], out=offs[1:])
         blob = b"".join(raw)
-        stride = 256
+        stride = (self.max_len + 31) // 32 * 32
         ids = np.empty((B, stride), np.int32)
         lens = np.empty(B, np.int32)
         fb = np.empty(B, np.uint8)
@@ -143,7 +143,7 @@ class _Base:
             ids[b, len(r) :] = self.pad_id
             lens[b] = len(r)
         longest = int(lens.max()) if B else 2
-        S = min(256, (max(longest, 2) + 31) // 32 * 32)
+        S = (max(longest, 2) + 31) // 32 * 32
         return np.ascontiguousarray(ids[:, :S]), lens
 
     def __del__(self):
@@ -168,7 +168,7 @@ class WordPieceTokenizer(_Base):
         self._vocab_list = list(vocab)
 
     @classmethod
-    def from_dir(cls, path):
+    def from_dir(cls, path, max_len=256):
         """`vocab.txt` of a local model directory, cased or not as its `tokenizer_config.json` says (without it: not).
         Another tokeniser than BERT's, or BERT's with other switches, is a ValueError."""
         raw = read_json(path, "tokenizer_config.json")
@@ -178,7 +178,7 @@ class WordPieceTokenizer(_Base):
                 raise ValueError(f"{os.path.join(path, 'tokenizer_config.json')}: {key} {raw[key]!r} is not the tokeniser built here ({ours[0]})")
         if read_json(path, "sentence_bert_config.json").get("do_lower_case") and not lower:
             raise ValueError(f"{path}: lower case in front of a cased tokeniser is not built here")
-        return cls(os.path.join(path, "vocab.txt"), lower=bool(lower))
+        return cls(os.path.join(path, "vocab.txt"), lower=bool(lower), max_len=max_len)
 
     def _vocab_blob(self):
         return "\n".join(self._vocab_list).encode("utf-8", "surrogatepass")

@@ -14,7 +14,7 @@ Linear weights are [out, in] (y = x @ w.T + b), as BERT stores them.
 import json
 import os
 import warnings
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 import numpy as np
 
@@ -47,7 +47,14 @@ class EncoderConfig:
         for key, want in (("model_type", "bert"), ("hidden_act", "gelu"), ("position_embedding_type", "absolute")):
             if raw.get(key, want) != want:
                 raise ValueError(f"{file}: {key} {raw[key]!r} is not the encoder built here ({want})")
-        return cls(**{ours: type(getattr(cls, ours))(raw[theirs]) for ours, theirs in keys.items() if theirs in raw})
+        cfg = cls(**{ours: type(getattr(cls, ours))(raw[theirs]) for ours, theirs in keys.items() if theirs in raw})
+        # texts are cut where the directory says, at 256 tokens where it does not, and never behind the last position
+        length = read_json(path, "sentence_bert_config.json").get("max_seq_length") or read_json(path, "tokenizer_config.json").get("model_max_length") or cfg.max_seq
+        length = min(int(length), cfg.max_pos)
+        if length > 256 and not cfg.packs:
+            warnings.warn(f"{path}: texts are cut at 256 tokens, the longest this geometry's kernels take, not at {length}", stacklevel=2)
+            length = 256
+        return replace(cfg, max_seq=length)
 
 
 def read_json(path, *names):

@@ -71,3 +71,68 @@ def test_tokeniser_is_cased_where_the_directory_says_so(tmp_path):
     _write(tmp_path, **{"tokenizer_config.json": {"do_lower_case": False}, "sentence_bert_config.json": {"do_lower_case": True}})
     with pytest.raises(ValueError, match="lower case"):
         WordPieceTokenizer.from_dir(str(tmp_path))
+
+
+WIDE = {"model_type": "bert", "vocab_size": 8, "hidden_size": 128, "num_hidden_layers": 1, "num_attention_heads": 2, "intermediate_size": 64}
+
+
+@pytest.mark.parametrize("files,want", [
+    ({}, 256),
+    ({"sentence_bert_config.json": {"max_seq_length": 128}}, 128),
+    ({"sentence_bert_config.json": {"max_seq_length": 512}, "tokenizer_config.json": {"model_max_length": 100}}, 512),
+    ({"tokenizer_config.json": {"model_max_length": 400}}, 400),
+    ({"tokenizer_config.json": {"model_max_length": 10**30}}, 512),
+    ({"config.json": {**WIDE, "max_position_embeddings": 100}}, 100),
+    ({"config.json": {**WIDE, "max_position_embeddings": 600}, "sentence_bert_config.json": {"max_seq_length": 600}}, 600),
+])
+def test_texts_are_cut_where_the_directory_says(tmp_path, files, want):
+    (tmp_path / "vocab.txt").write_text("\n".join(VOCAB) + "\n", encoding="utf-8")
+    _write(tmp_path, **{"config.json": {**WIDE, "max_position_embeddings": 512}})
+    _write(tmp_path, **files)
+    cfg = W.EncoderConfig.from_dir(str(tmp_path))
+    assert cfg.packs and cfg.max_seq == want
+    tok = WordPieceTokenizer.from_dir(str(tmp_path), cfg.max_seq)
+    texts = ["server " * 1000, "server", "server " * (want - 3), "server " * (want - 2), "server " * (want - 1)]
+    for ids, lens in (tok.encode_batch(texts), tok.encode_batch_python(texts)):
+        assert lens.tolist() == [want, 3, want - 1, want, want] and ids.shape[1] == (want + 31) // 32 * 32
+        assert ids[0].tolist() == [2] + [4] * (want - 2) + [3] + [0] * (ids.shape[1] - want)
+
+
+def test_the_built_in_geometry_cuts_at_256_and_says_so(tmp_path):
+    _write(tmp_path, **{"sentence_bert_config.json": {"max_seq_length": 128}})
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        assert W.EncoderConfig.from_dir(str(tmp_path)).max_seq == 128
+    _write(tmp_path, **{"sentence_bert_config.json": {"max_seq_length": 512}})
+    with pytest.warns(UserWarning, match="256 tokens"):
+        assert W.EncoderConfig.from_dir(str(tmp_path)).max_seq == 256
+
+
+def test_the_embedding_function_cuts_at_the_directorys_length(tmp_path, monkeypatch):
+    """HrsEmbeddingFunction up to the encoder's call, which is recorded instead."""
+    import torch
+
+    from hybrid_rag_system_amd import store
+
+    seen = []
+
+    class Recorder:
+        device = torch.device("cpu")
+
+        def encoder(self, weights, cfg):
+            self.cfg = cfg
+            return self
+
+        def encode_packed(self, ids, offs, max_len):
+            seen.append((ids, offs, max_len))
+            return torch.zeros(len(offs) - 1, self.cfg.hidden)
+
+    eng = Recorder()
+    monkeypatch.setattr(store, "engine", lambda: eng)
+    monkeypatch.setattr(store.W, "load_safetensors", lambda path, cfg: {})
+    (tmp_path / "model.safetensors").write_bytes(b"")
+    (tmp_path / "vocab.txt").write_text("\n".join(VOCAB) + "\n", encoding="utf-8")
+    _write(tmp_path, **{"config.json": {**WIDE, "max_position_embeddings": 40}})
+    assert store.HrsEmbeddingFunction(model_dir=str(tmp_path)).embed_tensor(["server " * 300, "server"]).shape == (2, 128)
+    ids, offs, longest = seen.pop()
+    assert offs.tolist() == [0, 3, 43] and longest == 40 and len(ids) == 43  # nothing stands behind the last position
