@@ -477,6 +477,13 @@ class Engine:
         if shape is not None and tuple(t.shape) != shape:
             raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {shape}")
 
+    @staticmethod
+    def _forward_only(*tensors):
+        """These operators leave no graph: an input whose gradient is being recorded would silently lose it."""
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError("an input requires a gradient, and the engine's operators are forward only: call them under torch.no_grad(), or detach the input")
+
     def _rows(self, name, t, dtype, n=None):
         """[.., N] with its elements next to each other as rows: -> the [rows, N] view (no copy)."""
         self._check(name, t, dtype)
@@ -523,10 +530,13 @@ class Engine:
         """act(x @ weight.T + bias) + residual in one kernel (hrs_linear): x [.., K] and weight [N, K] bf16 or fp16, bias
         fp32 [N], residual [.., N] as x; activation "none", "relu", "gelu" (erf), "gelu_tanh", "silu" or "tanh".  Rows may
         lie at any stride.  Sums, bias, activation and residual in fp32, one rounding.  out (as the result) may be
-        residual, not x or weight.  Forward only."""
+        residual, not x or weight.  Forward only: an
+        input that requires a gradient is refused while gradients are recorded."""
         dtype = x.dtype
         if dtype not in (torch.bfloat16, torch.float16):
             raise ValueError(f"x must be bfloat16 or float16, not {dtype}")
+        if torch.is_grad_enabled():
+            self._forward_only(x, weight, bias, residual, out)
         act = N.ACTIVATIONS.get(activation)
         if act is None:
             raise ValueError(f"unknown activation {activation!r}: one of {', '.join(N.ACTIVATIONS)}")
@@ -549,10 +559,13 @@ class Engine:
 
     def layer_norm(self, x, weight, bias=None, eps=1e-12, residual=None, out=None):
         """LayerNorm of x + residual over the last dimension (hrs_layer_norm): bf16, fp16 or fp32, weight and bias fp32
-        [N], statistics in fp32, one rounding.  Rows may lie at any stride; out may be x or residual.  Forward only."""
+        [N], statistics in fp32, one rounding.  Rows may lie at any stride; out may be x or residual.  Forward only, as
+        linear is."""
         dtype = x.dtype
         if dtype not in _TYPES:
             raise ValueError(f"x must be bfloat16, float16 or float32, not {dtype}")
+        if torch.is_grad_enabled():
+            self._forward_only(x, weight, bias, residual, out)
         if x.dim() < 1:
             raise ValueError("x has no dimension to normalise over")
         n = x.shape[-1]
@@ -580,10 +593,12 @@ class Engine:
         hides the keys behind a query, except the first prefix_lens[b] (int32 [B]).  Scores are scale q . k (scale
         D ** -0.5 where not given), capped to softcap tanh(. / softcap), with a bias by distance: -slopes[h] |j - p|, or
         bias_table[h, clamp(j - p, -R, R) + R] (fp32 [Hq, 2 R + 1]).  A query that sees no key gives zeros.
-        max_q and max_k (longest documents of a packed batch) only shape the launch.  -> as q, contiguous.  Forward only."""
+        max_q and max_k (longest documents of a packed batch) only shape the launch.  -> as q, contiguous.  Forward only, as linear is."""
         dtype = q.dtype
         if dtype not in (torch.bfloat16, torch.float16):
             raise ValueError(f"q must be bfloat16 or float16, not {dtype}")
+        if torch.is_grad_enabled():
+            self._forward_only(q, k, v, slopes, bias_table, out)
         packed = q_offs is not None
         nd = 3 if packed else 4
         strides = []

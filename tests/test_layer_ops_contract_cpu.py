@@ -4,8 +4,10 @@ import ctypes as C
 import struct
 
 import pytest
+import torch
 
 from hybrid_rag_system_amd import _native as N
+from hybrid_rag_system_amd.engine import Engine
 from test_layer_ops_cpu import _attention_args, _p
 
 CTX = C.create_string_buffer(4096)
@@ -31,3 +33,25 @@ def test_workspace_size_does_not_depend_on_addresses(shape):
         if need:
             a = _attention_args(**shape, workspace=_p(2048).value, workspace_bytes=given)
             assert N.lib().hrs_attention(CTX, C.byref(a), None) == -1 and f"workspace of {need} bytes" in N.last_error()
+
+
+def test_inputs_that_require_a_gradient_are_refused():
+    """While gradients are recorded, by name; without recording the same call goes on (here to the check of its device)."""
+    eng = object.__new__(Engine)
+    eng.device, eng._ctx = torch.device("cuda", 0), None
+    b = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)
+    calls = {
+        "linear": (eng.linear, dict(x=b(2, 8), weight=b(4, 8), bias=torch.zeros(4), residual=b(2, 4))),
+        "layer_norm": (eng.layer_norm, dict(x=b(2, 8), weight=torch.zeros(8), bias=torch.zeros(8), residual=b(2, 8))),
+        "attention": (eng.attention, dict(q=b(1, 2, 1, 8), k=b(1, 2, 1, 8), v=b(1, 2, 1, 8), slopes=torch.zeros(1))),
+        "attention with a table": (eng.attention, dict(q=b(1, 2, 1, 8), k=b(1, 2, 1, 8), v=b(1, 2, 1, 8), bias_table=torch.zeros(1, 3))),
+    }
+    for name, (call, kw) in calls.items():
+        for arg in kw:
+            with_grad = {**kw, arg: kw[arg].clone().requires_grad_()}
+            with pytest.raises(ValueError, match="requires a gradient"):
+                call(**with_grad)
+            with torch.no_grad(), pytest.raises(ValueError, match="must be on cuda:0|bias_table"):
+                call(**with_grad)
+        with pytest.raises(ValueError, match="must be on cuda:0|bias_table"):
+            call(**kw)
