@@ -587,22 +587,28 @@ extern "C" int hrs_linear(hrs_ctx* ctx, int dtype, const void* x_dev, int64_t ld
     hrs_device_scope dev(ctx->device);
     HRS_CHECK_HIP(dev.err);
     LinearArgs a;
-    a.w = w_dev;
-    a.bias = bias_dev;
     a.ldx = ldx;
     a.ldw = ldw;
     a.ldr = ldr;
     a.ldy = ldy;
-    a.N = (int)N;
     a.K = (int)K;
-    const int64_t most = 1 << 22;  // rows per launch: a grid holds less than 2^32 threads
-    for (int64_t m0 = 0; m0 < M; m0 += most) {
-        a.x = (const char*)x_dev + m0 * ldx * 2;
-        a.y = (char*)y_dev + m0 * ldy * 2;
-        a.resid = resid_dev ? (const char*)resid_dev + m0 * ldr * 2 : nullptr;
-        a.M = M - m0 < most ? M - m0 : most;
-        const int rc = dtype == HRS_TYPE_BF16 ? launch_linear_act<__bf16>(ctx, a, act, (hipStream_t)stream) : launch_linear_act<_Float16>(ctx, a, act, (hipStream_t)stream);
-        if (rc) return rc;
+    // Rows and features per launch: a grid holds less than 2^32 threads, of which a kernel takes at most 64 per feature (up to
+    // 16 tokens) or one per 32 results.
+    const int64_t most_n = 1 << 25;
+    for (int64_t n0 = 0; n0 < N; n0 += most_n) {
+        a.N = (int)(N - n0 < most_n ? N - n0 : most_n);
+        a.w = (const char*)w_dev + n0 * ldw * 2;
+        a.bias = bias_dev ? bias_dev + n0 : nullptr;
+        int64_t most = (1ll << 36) / a.N;
+        if (most > 1 << 22) most = 1 << 22;
+        for (int64_t m0 = 0; m0 < M; m0 += most) {
+            a.x = (const char*)x_dev + m0 * ldx * 2;
+            a.y = (char*)y_dev + (m0 * ldy + n0) * 2;
+            a.resid = resid_dev ? (const char*)resid_dev + (m0 * ldr + n0) * 2 : nullptr;
+            a.M = M - m0 < most ? M - m0 : most;
+            const int rc = dtype == HRS_TYPE_BF16 ? launch_linear_act<__bf16>(ctx, a, act, (hipStream_t)stream) : launch_linear_act<_Float16>(ctx, a, act, (hipStream_t)stream);
+            if (rc) return rc;
+        }
     }
     return HRS_OK;
 }

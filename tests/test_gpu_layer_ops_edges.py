@@ -153,3 +153,18 @@ def test_attention_many_small_weights_are_not_lost(eng, queries, heads, aligned,
     # tile of 32 keys at least with one rounding of 2^-24, the products 16 keys with one of 2^-23 at most.
     tol = LO.half_step(TYPES[t]) + (n / 32 + 2 * n / 16) * 2.0**-24 + 2 * mass * 2.0**-18
     assert (got - (1 - mass) / (1 + mass)).abs().max() <= tol
+
+
+# ---- very wide outputs -------------------------------------------------------------------------------
+@pytest.mark.parametrize("m,k,ld", [(1, 8, 8), (3, 40, 1), (2, 2048, 8), (17, 8, 8)])
+def test_linear_more_features_than_one_launch_takes(eng, m, k, ld):
+    """2^27 features and some: the rows of W overlap, so that they need little memory.  Equal to the products of their parts."""
+    n = (1 << 27) + 40
+    base, x = torch.randn(n * ld + k, device="cuda").bfloat16(), torch.randn(m, k, device="cuda").bfloat16()
+    w, b, r = base.as_strided((n, k), (ld, 1)), torch.randn(n, device="cuda"), torch.randn(m, n, device="cuda").bfloat16()
+    y = eng.linear(x, w, b, "relu", r)
+    for at in (0, (1 << 25) - 100, (1 << 26) - 100, 3 * (1 << 25) - 100, n - 200):
+        part = slice(at, at + 200)
+        assert torch.equal(y[:, part], eng.linear(x, w[part], b[part], "relu", r[:, part])), at
+    eng.linear(x, w, b, "relu", r, out=r)  # in place of the residual
+    assert torch.equal(r, y)
