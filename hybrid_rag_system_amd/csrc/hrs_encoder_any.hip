@@ -272,7 +272,12 @@ int hrs_encoder_any_run(hrs_ctx* ctx, hrs_encoder_any* e, const int32_t* ids_dev
             return rc;
     }
     const int pieces = H / 8, phases = pieces >= 256 ? 1 : 256 / pieces;
-    hipLaunchKernelGGL(k_pool_rows, dim3(B), dim3(256), (phases * H + 4) * sizeof(float), st, x, offs_dev, lens_dev, S, (int)T, H, out_dev);
+    const int most = 1 << 23;  // documents per launch: a grid holds less than 2^32 threads
+    for (int b0 = 0; b0 < B; b0 += most) {
+        const int *offs = offs_dev ? offs_dev + b0 : nullptr, *lens = lens_dev ? lens_dev + b0 : nullptr;
+        hipLaunchKernelGGL(k_pool_rows, dim3(B - b0 < most ? B - b0 : most), dim3(256), (phases * H + 4) * sizeof(float), st, offs_dev ? x : x + (size_t)b0 * S * H, offs, lens, S, (int)T, H,
+                           out_dev + (size_t)b0 * H);
+    }
     HRS_CHECK_HIP(hipGetLastError());
     return HRS_OK;
 }
