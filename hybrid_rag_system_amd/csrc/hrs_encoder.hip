@@ -1312,11 +1312,12 @@ extern "C" int hrs_encoder_load(hrs_ctx* ctx, const hrs_encoder_config* cfg, con
     const bool built = cfg->hidden == ENC_H && cfg->heads == ENC_HEADS && cfg->inter > 0 && cfg->inter % G_BN == 0 && cfg->inter % G_BK == 0 && cfg->inter <= 8 * ENC_H &&
                        cfg->layers >= 1 && cfg->layers <= 16;
     if (!built) {
-        HRS_REQUIRE(cfg->layers >= 1 && cfg->layers <= 256, "hrs_encoder_load: layers=%d outside [1, 256]", cfg->layers);
+        int rc = hrs_encoder_any_check(cfg);  // (before w, whose length the geometry says)
+        if (rc) return rc;
         for (int t = 0; t < 5 + 16 * cfg->layers; ++t) HRS_REQUIRE(w[t] != nullptr, "hrs_encoder_load: weight tensor %d is null", t);
         HRS_CHECK_HIP(hipSetDevice(ctx->device));
         hrs_encoder_any* any = nullptr;
-        const int rc = hrs_encoder_any_load(ctx, cfg, w, stream, &any);
+        rc = hrs_encoder_any_load(cfg, w, stream, &any);
         if (rc) return rc;
         hrs_encoder* e = new hrs_encoder();
         e->cfg = *cfg;

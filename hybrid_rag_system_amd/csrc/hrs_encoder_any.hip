@@ -188,14 +188,17 @@ static int any_load(hrs_encoder_any* e, const float* const* w, hipStream_t st) {
     return HRS_OK;
 }
 
-int hrs_encoder_any_load(hrs_ctx* ctx, const hrs_encoder_config* cfg, const float* const* w, void* stream, hrs_encoder_any** out) {
-    (void)ctx;
+int hrs_encoder_any_check(const hrs_encoder_config* cfg) {
     HRS_REQUIRE(cfg->hidden >= 8 && cfg->hidden <= 4096 && cfg->hidden % 8 == 0, "hrs_encoder_load: hidden=%d must be a multiple of 8 in [8, 4096]", cfg->hidden);
     HRS_REQUIRE(cfg->heads >= 1 && cfg->hidden % cfg->heads == 0 && cfg->hidden / cfg->heads % 8 == 0 && cfg->hidden / cfg->heads <= 256,
                 "hrs_encoder_load: hidden=%d over heads=%d is not a head width that is a multiple of 8, at most 256", cfg->hidden, cfg->heads);
     HRS_REQUIRE(cfg->inter >= 1 && cfg->inter <= (1 << 20), "hrs_encoder_load: intermediate size %d", cfg->inter);
     HRS_REQUIRE(cfg->layers >= 1 && cfg->layers <= 256, "hrs_encoder_load: layers=%d outside [1, 256]", cfg->layers);
     HRS_REQUIRE(cfg->vocab > 0 && cfg->max_pos > 0, "hrs_encoder_load: bad vocabulary / position table size");
+    return HRS_OK;
+}
+
+int hrs_encoder_any_load(const hrs_encoder_config* cfg, const float* const* w, void* stream, hrs_encoder_any** out) {
     hrs_encoder_any* e = new hrs_encoder_any();
     e->cfg = *cfg;
     e->layer.resize(cfg->layers);
@@ -208,8 +211,6 @@ int hrs_encoder_any_load(hrs_ctx* ctx, const hrs_encoder_config* cfg, const floa
     *out = e;
     return HRS_OK;
 }
-
-const hrs_encoder_config* hrs_encoder_any_config(const hrs_encoder_any* e) { return &e->cfg; }
 
 // offs_dev (packed, T rows) or lens_dev (padded, T = B S rows); longest: of a document (packed: a hint)
 int hrs_encoder_any_run(hrs_ctx* ctx, hrs_encoder_any* e, const int32_t* ids_dev, const int32_t* offs_dev, const int32_t* lens_dev, int B, int S, int64_t T, int64_t longest, float* out_dev,

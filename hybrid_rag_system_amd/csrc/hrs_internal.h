@@ -337,8 +337,8 @@ int hrs_exact_static_init(int device);
 
 // Encoders of other geometries than the one hrs_encoder.hip is built for (hrs_encoder_any.hip).
 struct hrs_encoder_any;
-int hrs_encoder_any_load(hrs_ctx* ctx, const hrs_encoder_config* cfg, const float* const* w, void* stream, hrs_encoder_any** out);
+int hrs_encoder_any_check(const hrs_encoder_config* cfg);  // whether such a geometry is built
+int hrs_encoder_any_load(const hrs_encoder_config* cfg, const float* const* w, void* stream, hrs_encoder_any** out);
 void hrs_encoder_any_release(hrs_encoder_any* e);
-const hrs_encoder_config* hrs_encoder_any_config(const hrs_encoder_any* e);
 int hrs_encoder_any_run(hrs_ctx* ctx, hrs_encoder_any* e, const int32_t* ids_dev, const int32_t* offs_dev, const int32_t* lens_dev,
                         int B, int S, int64_t T, int64_t longest, float* out_dev, hipStream_t st);

@@ -55,3 +55,13 @@ def test_inputs_that_require_a_gradient_are_refused():
                 call(**with_grad)
         with pytest.raises(ValueError, match="must be on cuda:0|bias_table"):
             call(**kw)
+
+
+def test_a_geometry_that_is_not_built_is_refused_before_its_weights_are_read():
+    """w holds as many pointers as the geometry says; a refused one says nothing."""
+    w, out = (C.c_void_p * 8192)(), C.c_void_p()
+    good = dict(vocab=100, hidden=128, layers=1, heads=2, inter=64, max_pos=16, eps=1e-12)
+    for kw, word in ((dict(hidden=100, heads=4), "hidden=100"), (dict(hidden=8192), "hidden=8192"), (dict(heads=3), "heads=3"), (dict(inter=0), "intermediate"), (dict(layers=257), "layers=257"),
+                     (dict(layers=0), "layers=0"), (dict(vocab=0), "vocabulary"), (dict(max_pos=0), "position"), ({}, "weight tensor 0 is null")):
+        cfg = N.EncoderConfigC(**{**good, **kw})
+        assert N.lib().hrs_encoder_load(CTX, C.byref(cfg), w, None, C.byref(out)) == -1 and word in N.last_error(), N.last_error()
