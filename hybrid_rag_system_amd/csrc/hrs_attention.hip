@@ -67,12 +67,12 @@ __device__ __forceinline__ DocRange doc_range(const AttnArgs& a, int b) {
     return d;
 }
 
-// Where 16-byte piece p of row i lies in its row of DP elements.  K: 8 consecutive rows, same piece -> 8 bank groups.
+// Piece p of row i lies at piece p ^ swizzle of its row of DP elements.  K: 8 consecutive rows, same piece -> 8 bank groups.
 // V: 4 consecutive rows, two pieces -> 8 bank groups.
 template <int DP>
-__device__ __forceinline__ int place_k(int i, int p) { return DP == 32 ? p ^ ((i >> 1) & 3) : p ^ (i & 7); }
+__device__ __forceinline__ int swizzle_k(int i) { return DP == 32 ? (i >> 1) & 3 : i & 7; }
 template <int DP>
-__device__ __forceinline__ int place_v(int i, int p) { return DP == 32 ? p ^ (i & 2) : p ^ ((i & 3) << 1); }
+__device__ __forceinline__ int swizzle_v(int i) { return DP == 32 ? i & 2 : (i & 3) << 1; }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 // Four rows of 16 elements, one row per four lanes (each lane names 8 bytes); lane l of 16 receives column l of the four.
@@ -186,8 +186,8 @@ __global__ __launch_bounds__(256) void k_attend_any(AttnArgs a) {
                 const int i = id2 / PPR, p = id2 % PPR;
                 const int64_t j = j0 + i;
                 const int left = j < dr.lk ? a.dim - p * 8 : 0;  // what stands behind the document is never read: zeros
-                *(x8*)(kl + i * (DP * 2) + place_k<DP>(i, p) * 16) = load8_any<T>(kbase + j * a.k_st + p * 8, left);
-                *(x8*)(vl + i * (DP * 2) + place_v<DP>(i, p) * 16) = load8_any<T>(vbase + j * a.v_st + p * 8, left);
+                *(x8*)(kl + i * (DP * 2) + (p ^ swizzle_k<DP>(i)) * 16) = load8_any<T>(kbase + j * a.k_st + p * 8, left);
+                *(x8*)(vl + i * (DP * 2) + (p ^ swizzle_v<DP>(i)) * 16) = load8_any<T>(vbase + j * a.v_st + p * 8, left);
             }
             __syncthreads();
             f32x16 s[NB];
@@ -196,7 +196,7 @@ __global__ __launch_bounds__(256) void k_attend_any(AttnArgs a) {
                 s[n] = (f32x16)(0.f);
                 const int i = n * 32 + c32;
 #pragma unroll
-                for (int t = 0; t < NS; ++t) s[n] = mfma32(*(const x8*)(kl + i * (DP * 2) + place_k<DP>(i, 2 * t + h) * 16), qf[t], s[n]);
+                for (int t = 0; t < NS; ++t) s[n] = mfma32(*(const x8*)(kl + i * (DP * 2) + ((2 * t + h) ^ swizzle_k<DP>(i)) * 16), qf[t], s[n]);
             }
             float top = -INFINITY;
 #pragma unroll
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(256) void k_attend_any(AttnArgs a) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const int key = t * 16 + e * 8 + 4 * h + ((lane & 15) >> 2), col = i * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-                        vf.half[e] = lds_read_tr(vl + key * (DP * 2) + place_v<DP>(key, col >> 3) * 16 + (col & 7) * 2);
+                        vf.half[e] = lds_read_tr(vl + key * (DP * 2) + ((col >> 3) ^ swizzle_v<DP>(key)) * 16 + (col & 7) * 2);
                     }
                     acc[i] = mfma32(vf.all, pf[t], acc[i]);
                 }
@@ -264,11 +264,6 @@ __global__ __launch_bounds__(256) void k_attend_any(AttnArgs a) {
 }
 
 // ---- aligned operands: K and V by LDS-DMA --------------------------------------------------------------
-template <int DP>
-__device__ __forceinline__ int swizzle_k(int i) { return DP == 32 ? (i >> 1) & 3 : i & 7; }
-template <int DP>
-__device__ __forceinline__ int swizzle_v(int i) { return DP == 32 ? i & 2 : (i & 3) << 1; }
-
 // A row of the tile and what it is allowed to see.
 struct RowPlace {
     int row;  // row / group: token, row % group: head of this key head's group

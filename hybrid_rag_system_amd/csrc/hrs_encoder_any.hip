@@ -18,12 +18,6 @@ struct hrs_encoder_any {
     hrs_workspace ws;
 };
 
-__device__ __forceinline__ float sum_of_wave(float v) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
-    return v;
-}
-
 // First row and length of document b, inside the T rows.
 struct EncDoc {
     int row, len;
@@ -66,7 +60,7 @@ __global__ __launch_bounds__(256) void k_embed_norm(const int* __restrict__ ids,
                 s += z[j][e];
             }
         }
-        const float mean = sum_of_wave(s) / (float)H;
+        const float mean = wave_sum(s) / (float)H;
         float v = 0.f;
 #pragma unroll
         for (int j = 0; j < CH; ++j)
@@ -75,7 +69,7 @@ __global__ __launch_bounds__(256) void k_embed_norm(const int* __restrict__ ids,
                 const float dv = z[j][e] - mean;
                 v += (j * 64 + lane) * 8 < H ? dv * dv : 0.f;
             }
-        const float rstd = 1.f / sqrtf(sum_of_wave(v) / (float)H + eps);
+        const float rstd = 1.f / sqrtf(wave_sum(v) / (float)H + eps);
 #pragma unroll
         for (int j = 0; j < CH; ++j) {
             const int c = (j * 64 + lane) * 8;
@@ -118,7 +112,7 @@ __global__ __launch_bounds__(256) void k_pool_rows(const __bf16* __restrict__ x,
         sums[c] = s;  // (own column: nobody else reads it before the next barrier)
         q = fmaf(s, s, q);
     }
-    q = sum_of_wave(q);
+    q = wave_sum(q);
     float* norms = sums + phases * H;
     if ((threadIdx.x & 63) == 0) norms[threadIdx.x >> 6] = q;
     __syncthreads();

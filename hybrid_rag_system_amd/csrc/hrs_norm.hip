@@ -17,12 +17,6 @@ struct NormArgs {
     float eps;
 };
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
-    return v;
-}
-
 // 8 elements of z at column c of a row, as fp32 (zero where the row has ended)
 template <typename T>
 __device__ __forceinline__ void load_z(const T* x, const T* r, int c, int N, float (&z)[8]) {

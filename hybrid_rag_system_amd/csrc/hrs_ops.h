@@ -44,6 +44,13 @@ __device__ __forceinline__ float add_pair(vec_of<_Float16>::x2 v, float c) {
     return __builtin_amdgcn_fdot2(v, one, c, false);
 }
 
+// v over the wave's lanes
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+    return v;
+}
+
 // Every earlier load of this wave has arrived, every earlier LDS access of it is done; then the workgroup's barrier.
 __device__ __forceinline__ void wait_all_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
