@@ -381,7 +381,7 @@ struct Attend {
         }
         if constexpr (RAMP) {
             // The scores are read behind a branch here, and the compiler has left a read too close behind the last product
-            // on such a path (three of the eleven wait states that the result of a 32 x 32 product needs).
+            // on such a path (three of the twelve wait states that the result of a 32 x 32 product needs).
             __builtin_amdgcn_sched_barrier(0);
             asm volatile("s_nop 11");
             __builtin_amdgcn_sched_barrier(0);

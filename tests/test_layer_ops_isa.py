@@ -93,3 +93,105 @@ def test_no_spills_and_no_packed_fp32(code, source):
     spills = [line for line in code[source] if re.match(r"\s+\.vgpr_spill_count:\s+[1-9]", line)]
     assert not spills
     assert not [line for line in code[source] if re.search(r"\bv_pk_(add|mul|fma)_f32", line)]
+
+
+def _walk(lines, need_of):
+    """Every read of a matrix instruction's result along every path behind it -> (instructions, reads that come early)."""
+    checked, early = 0, []
+    for name, body in _kernels(lines).items():
+        labels = {t: i for i, (is_label, t) in enumerate(body) if is_label}
+        for i, (is_label, text) in enumerate(body):
+            if is_label or not text.startswith("v_mfma"):
+                continue
+            checked += 1
+            need, result = need_of(text), _registers(text.split(",")[0])
+            paths, seen = [(i + 1, 0)], {}
+            while paths:
+                j, waited = paths.pop()
+                while j < len(body) and waited < need and seen.get(j, need) > waited:
+                    seen[j] = waited
+                    is_label, ins = body[j]
+                    j += 1
+                    if is_label:
+                        continue
+                    op = ins.split()[0]
+                    if op == "s_endpgm" or (op.startswith("v_mfma") and _registers(ins.split(",")[0]) == result):
+                        break
+                    if not op.startswith(("v_mfma", "s_")) and _registers(ins) & result:
+                        early.append((name, text, ins, waited, need))
+                        break
+                    if op == "s_branch" or op.startswith("s_cbranch"):
+                        paths.append((labels[ins.split()[-1]], waited + 1))
+                        if op == "s_branch":
+                            break
+                    waited += int(ins.split()[1], 0) + 1 if op == "s_nop" else 1
+    return checked, early
+
+
+_PROBE = """
+#include <hip/hip_runtime.h>
+typedef __bf16 x8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16 __attribute__((ext_vector_type(16)));
+__global__ void probe_32x32x16(const x8* a, float* out) {
+    f16 c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[threadIdx.x], a[threadIdx.x + 64], (f16)(0.f), 0, 0, 0);
+    out[threadIdx.x] = c[0] + c[15];
+}
+__global__ void probe_16x16x32(const x8* a, float* out) {
+    f4 c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[threadIdx.x], a[threadIdx.x + 64], (f4)(0.f), 0, 0, 0);
+    out[threadIdx.x] = c[0] + c[3];
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def wait_states(tmp_path_factory):
+    """Shape -> wait states that this compiler itself puts between such an instruction and the first vector read of its
+    result, in a straight line."""
+    d = tmp_path_factory.mktemp("probe")
+    (d / "probe.hip").write_text(_PROBE)
+    subprocess.run([HIPCC] + FLAGS + ["--cuda-device-only", "-S", str(d / "probe.hip"), "-o", str(d / "probe.s")], check=True, stderr=subprocess.DEVNULL)
+    found = {}
+    for body in _kernels((d / "probe.s").read_text().splitlines()).values():
+        at = next(i for i, (_, t) in enumerate(body) if t.startswith("v_mfma"))
+        result, waited = _registers(body[at][1].split(",")[0]), 0
+        for _, ins in body[at + 1 :]:
+            op = ins.split()[0]
+            if not op.startswith("s_") and _registers(ins) & result:
+                break
+            waited += int(ins.split()[1], 0) + 1 if op == "s_nop" else 1
+        found[re.search(r"\d+x\d+x\d+", body[at][1]).group()] = waited
+    return found
+
+
+def test_wait_states_of_the_compiler(wait_states):
+    """8 passes of four cycles and 3 more for the 32 x 32 x 16 product, 4 and 3 for the 16 x 16 x 32 one, and the read's own."""
+    assert wait_states == {"32x32x16": 12, "16x16x32": 8}
+
+
+@pytest.mark.parametrize("source", ["hrs_linear.hip", "hrs_attention.hip"])
+def test_results_rest_as_long_as_the_compiler_waits(code, wait_states, source):
+    checked, early = _walk(code[source], lambda text: wait_states[re.search(r"\d+x\d+x\d+", text).group()])
+    assert checked > 1000 and not early, early[:3]
+
+
+def test_walk_catches_an_early_read():
+    """The walk itself: a read behind a branch, one wait state too early, and the same one further on."""
+    text = "_Z1kPf:\n v_mfma_f32_32x32x16_bf16 v[0:15], v[16:19], v[20:23], 0\n s_cbranch_scc1 .LBB0_2\n s_nop 11\n v_add_f32_e32 v20, v0, v1\n s_endpgm\n.LBB0_2:\n s_nop %d\n v_add_f32_e32 v20, v0, v15\n s_endpgm\n.Lfunc_end0:\n"
+    assert _walk((text % 10).splitlines(), lambda t: 12) == (1, [])
+    checked, early = _walk((text % 9).splitlines(), lambda t: 12)
+    assert checked == 1 and early[0][3:] == (11, 12)
+
+
+def test_flags_are_the_librarys():
+    """FLAGS and SOURCES against what make would run."""
+    plan = subprocess.run(["make", "-n", "-B", "-C", CSRC], check=True, capture_output=True, text=True).stdout
+    for source in SOURCES:
+        line = next(l for l in plan.splitlines() if f"-c {source} " in l)
+        assert [f for f in line.split()[1:] if f not in ("-fPIC", "-Wall", "-Wno-unused-function", "-c", source, "-o", source.replace(".hip", ".o"))] == FLAGS, line
+
+
+def test_other_kernels_have_no_matrix_instructions():
+    """What SOURCES leaves out of the encoder of other geometries has nothing to wait for."""
+    with open(os.path.join(CSRC, "hrs_encoder_any.hip")) as f:
+        assert "mfma" not in f.read()
