@@ -130,8 +130,8 @@ __device__ __forceinline__ float score2(const AttnArgs& a, float s, float slope2
 
 // ---- any alignment, any table ------------------------------------------------------------------------
 // 128 rows per workgroup, 32 per wave; pieces of K and V pass through registers one by one and the table is read from
-// memory.  Two to four times slower than the kernels below (two documents of 8192 tokens, 16 heads of 64, slope: 1.76 ms
-// against 0.75): the way for operands that cannot be fetched in aligned 16-byte pieces.
+// memory.  Two to four times slower than the kernels below (two documents of 8192 tokens, 16 heads of 64, slope: 1.57 ms
+// against 0.74): the way for operands that cannot be fetched in aligned 16-byte pieces.
 template <typename T, int DP, int BIAS, bool CAP>
 __global__ __launch_bounds__(256) void k_attend_any(AttnArgs a) {
     typedef typename vec_of<T>::x8 x8;
@@ -634,8 +634,8 @@ __device__ __forceinline__ float inverse(float l) { return l > 0.f || l != l ? 1
 
 // ---- many rows: 128 per workgroup, 32 per wave ---------------------------------------------------------
 // All four waves read the tiles of 64 keys (32 for heads wider than 128) that they fetch together, two buffers deep.
-// Two documents of 8192 tokens, 16 heads of 64: 0.64 ms, 0.85 PFLOP/s; with a slope 0.75; causal 0.35; 8 heads of 128: 0.56 ms,
-// 0.97 PFLOP/s, capped 0.63.  Bound by the sum of matrix and vector work: per 64 keys x 32 rows x 64 a SIMD spends 512
+// Two documents of 8192 tokens, 16 heads of 64: 0.63 ms, 0.87 PFLOP/s; with a slope 0.74 (0.86 where the inputs are not
+// those of the call before, still in the caches); causal 0.35; 8 heads of 128: 0.555 ms, 0.99 PFLOP/s, capped 0.60.  Bound by the sum of matrix and vector work: per 64 keys x 32 rows x 64 a SIMD spends 512
 // cycles on products and about 900 on weights (32 exponentials of a quarter of the vector rate, 110 other operations), takes
 // 1190, and what one side saves the clock (1.9 GHz under this load) or the other side eats.  Built and not kept, all
 // within 3 %: 64 rows per wave (half the LDS reads, two independent softmax chains), four waves per SIMD, three tiles in
@@ -710,8 +710,8 @@ __global__ __launch_bounds__(256, DP <= 64 && !(BIAS == BIAS_SLOPE && !CAP) && C
 // ---- few rows: up to 32 per document and key head --------------------------------------------------------
 // The waves of a workgroup share the keys instead of the rows: wave w takes tiles w, w + NW, .. of 32 keys through an LDS
 // ring of its own, without a barrier, and the waves' sums meet at the end in a fixed order.
-// Bound by HBM: 8 documents of 32768 keys, 8 key heads of 128, 4 query heads each: 214 us, 5.0 TB/s, the rate of a copy;
-// lengths of 1 .. 32768 171 us (4.3 TB/s; the longest document's chunks end last), with a cap and a slope 204 us.
+// Bound by HBM: 8 documents of 32768 keys, 8 key heads of 128, 4 query heads each: 202 us, 5.3 TB/s, the rate of a copy;
+// lengths of 1 .. 32768 177 us (4.2 TB/s; the longest document's chunks end last), with a cap and a slope 205 us.
 template <typename T, int DP, int NW, int BIAS, int CAP, bool FIXED>
 __global__ __launch_bounds__(64 * NW) void k_attend_few(AttnArgs a) {
     constexpr int KT = 32, TILE = KT * DP * 2, ND = DP / 32, RING = 4 * TILE;
@@ -891,7 +891,9 @@ static int launch_form(hrs_ctx* ctx, const AttnArgs& a, const AttnPlan& p, hipSt
         return launch_attend(ctx, once, k_attend_any<T, DP, BIAS, CAP>, 256, 0, (int64_t)a.batch * a.kv_heads * a.tiles, a, st);
     }
     // Capped scores without a bias lie within +-cap: in bf16, whose range is that of fp32, the weights need no running
-    // maximum (2^+-80, their sum over 2^30 keys and its product with v stay inside fp32).
+    // maximum.  They are 2^+-80 at most, so that |v| times the number of keys may reach 2^48 and |v| may fall to 2^-46 before
+    // the sums leave fp32 (documented).  Two documents of 8192 tokens, 16 heads of 64: 795 us, 912 with the maximum; 8 heads
+    // of 128, 4096 tokens, causal: 172 and 184.
     if constexpr (CAP && BIAS == BIAS_NONE && __is_same(T, __bf16)) {
         if (a.cap2 <= 80.f) return launch_fast<T, DP, BIAS, CAP_TO_64, true>(ctx, a, p, st);
     }
@@ -1003,7 +1005,9 @@ static AttnPlan plan_attention(hrs_ctx* ctx, const hrs_attention_args* p, AttnAr
     if (!plan.fast) return plan;
     plan.few = rows <= 32;
     // Many documents: one workgroup takes all rows of a document (it walks on while there are rows), since most would find
-    // none or few: 1024 ragged documents of up to 256 tokens, 16 heads: 375 us with two workgroups for each, 323 with one.
+    // none or few: 1024 ragged documents of up to 256 tokens, 16 heads of 64: 358 us with two workgroups for each, 320 with one;
+    // 600 of up to 512: 577 and 488; 2048 of up to 128, 12 heads, without a hint: 397 and 219; but 400 of up to 1000, 12 heads of
+    // 32: 547 and 560.
     const int64_t pairs = (int64_t)a.batch * a.kv_heads, enough = 16 * (int64_t)ctx->num_cu;
     if (!plan.few && pairs * a.tiles > enough && (a.q_offs || a.q_lens)) {
         const int64_t t = (enough + pairs - 1) / pairs;

@@ -288,10 +288,10 @@ __global__ __launch_bounds__(64 * WR * WC * KG) void k_linear_tile(LinearArgs a)
 // A half's place in LDS is free as soon as both groups have read it, and is filled again for two stages ahead in the
 // next phase: a piece has a whole stage (2048 cycles) to arrive, and every phase waits for the half that the next one
 // reads with a counted wait, 8 younger requests still in flight.
-// 8192^3: 755 us, 1.46 PFLOP/s (a large library product there: 0.69 ms, 1.58); per 1024 of depth a 65536 x 4096 product takes
+// 8192^3: 743 us, 1.48 PFLOP/s (a large library product there: 0.69 ms, 1.58); per 1024 of depth a 65536 x 4096 product takes
 // 336 us, as the library's does, and 150 us besides: 107 of them are its 537 MB of output at the card's copy rate, which
 // nothing here runs under, since all workgroups finish their tiles at about the same time.  Workgroups that stay and fetch
-// the next tile under their stores were built and took the same time (486 us either way).  gelu adds 97 us to the 487:
+// the next tile under their stores were built and took the same time (486 us either way).  gelu adds 86 us to the 485:
 // 13 vector operations per value with the matrix pipe idle.
 template <typename T, int ACT>
 __global__ __launch_bounds__(512, 2) void k_linear_wide(LinearArgs a) {

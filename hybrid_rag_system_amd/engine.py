@@ -595,7 +595,8 @@ class Engine:
         hides the keys behind a query, except the first prefix_lens[b] (int32 [B]).  Scores are scale q . k (scale
         D ** -0.5 where not given), capped to softcap tanh(. / softcap), with a bias by distance: -slopes[h] |j - p|, or
         bias_table[h, clamp(j - p, -R, R) + R] (fp32 [Hq, 2 R + 1]).  A query that sees no key gives zeros.
-        max_q and max_k (longest documents of a packed batch) only shape the launch.  -> as q, contiguous.  Forward only, as linear is."""
+        max_q and max_k (longest documents of a packed batch) only shape the launch.  -> as q, contiguous.  Forward only, as linear is.
+        v must be finite where a query of the same 128 rows does not see it; include/hrs.h names the range of |v|."""
         dtype = q.dtype
         if dtype not in (torch.bfloat16, torch.float16):
             raise ValueError(f"q must be bfloat16 or float16, not {dtype}")

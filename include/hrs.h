@@ -262,7 +262,9 @@ typedef struct hrs_attention_args {
     size_t workspace_bytes;
 } hrs_attention_args;
 /* A query that sees no key gets zeros.  Weights are rounded to dtype before they meet v; sums and statistics are fp32.
- * k and v must be finite inside a document where a query of the same 128 rows may not see them (0 * inf is NaN). */
+ * v must be finite inside a document where a query of the same 128 rows may not see it (0 * inf is NaN).  Weights are
+ * not divided by their sum before they meet v: |v| times the number of keys stays below 2^110 (with a softcap of up to 55
+ * in bf16 without a bias: below 2^48, and |v| above 2^-46 where it is not 0). */
 int hrs_attention(hrs_ctx* ctx, const hrs_attention_args* args, void* stream);
 /* Bytes of workspace hrs_attention needs for these arguments (0 for most).  Of the pointers in args only whether they are
  * null counts: the answer is enough for any addresses. */
