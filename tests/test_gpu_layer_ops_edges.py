@@ -1,5 +1,6 @@
 """hrs_linear, hrs_attention and hrs_layer_norm at the ends of what their documentation allows: score caps of any size,
 infinities and NaN, weights far below a row's largest, very wide outputs.  Definitions and bounds: oracle/layer_oracle.py."""
+import itertools
 import math
 
 import pytest
@@ -168,3 +169,24 @@ def test_linear_more_features_than_one_launch_takes(eng, m, k, ld):
         assert torch.equal(y[:, part], eng.linear(x, w[part], b[part], "relu", r[:, part])), at
     eng.linear(x, w, b, "relu", r, out=r)  # in place of the residual
     assert torch.equal(r, y)
+
+
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+@pytest.mark.parametrize("queries,aligned", [(150, True), (7, True), (150, False)])
+def test_attention_keys_that_a_query_does_not_see_may_hold_anything(eng, queries, aligned, t):
+    """NaN and infinities in keys behind a query (v stays finite): with every bias and cap, as if they were zero."""
+    rnd = _gen(queries)
+    keys = 200
+    q, k, v = (rnd(1, n, 2, 64).to(TYPES[t]) for n in (queries, keys, keys))
+    for i, (cap, kw) in enumerate(itertools.product((0.0, 30.0, 100.0), ({}, {"slopes": torch.tensor([0.5, 0.01])}, {"table": rnd(2, 31)}))):
+        seen = keys - queries + 1 + i  # keys that query i sees
+        bad = k.clone()
+        bad[0, seen:, 0, i], bad[0, seen:, 1, 63] = float("nan"), float("inf")
+        dk, dv = bad.cuda(), v.cuda()
+        if not aligned:
+            dk, dv = _unaligned(dk), _unaligned(dv)
+        given = {("bias_table" if n == "table" else n): x.cuda() for n, x in kw.items()}
+        got = eng.attention(q.cuda(), dk, dv, causal=True, softcap=cap, **given)[0, : i + 1].cpu()
+        want, bound = LO.attention(q[0], k[0], v[0], queries, keys, causal=True, cap=cap, dtype=TYPES[t], **kw)
+        if i < queries:
+            _close(got, want[: i + 1], bound[: i + 1], (cap, list(kw)))
