@@ -515,9 +515,9 @@ template <int DP, int KT, int NWAVES>
 struct TileLoad {
     static constexpr int PPR = DP / 8, RPI = 64 / PPR, NI = KT / RPI / NWAVES;
     int kof[NI], vof[NI], row0;  // this lane's row of instruction j is row0 + j RPI
-    // lanes whose piece of K is inside the head's dimension, for instruction j % NM (the swizzle repeats every 8 rows)
-    static constexpr int NM = RPI >= 8 ? 1 : 8 / RPI < NI ? 8 / RPI : NI;
-    uint64_t in_head[NM];
+    int piece;                   // of K that instruction 0 fetches for this lane
+    // Whether instruction j fetches a piece of the head (its rows are j RPI further, a multiple of 8 or below it).
+    __device__ __forceinline__ bool in_head(const AttnArgs& a, int j) const { return (piece ^ (DP == 32 ? 0 : j * RPI & 7)) * 8 < a.dim; }
     __device__ __forceinline__ void open(const AttnArgs& a, int wave) {
         const int lane = threadIdx.x & 63;
         row0 = wave * NI * RPI + lane / PPR;
@@ -526,44 +526,58 @@ struct TileLoad {
             const int row = row0 + j * RPI, pk = (lane % PPR) ^ swizzle_k<DP>(row), pv = (lane % PPR) ^ swizzle_v<DP>(row);
             // (a piece of V behind the head's dimension repeats the first: it ends in columns not stored)
             kof[j] = row * (int)(a.k_st * 2) + pk * 16;
-            if (j < NM) in_head[j] = __ballot(pk * 8 < a.dim);
+            if (j == 0) piece = pk;
             vof[j] = row * (int)(a.v_st * 2) + (pv * 8 < a.dim ? pv * 16 : 0);
         }
     }
-    // Pieces of K behind the head's dimension are never fetched and meet zeros of q: zero in both buffers (0 times whatever
-    // stood there could be NaN).
-    __device__ __forceinline__ void blank_pads(const AttnArgs& a, uint32_t kl, int next, int wave) const {
+    // Pieces of K behind the head's dimension are never fetched and meet zeros of q: zero (0 times whatever stood there could
+    // be NaN), in the tile's first `rows` rows of one buffer or of both.
+    __device__ __forceinline__ void blank_pads(const AttnArgs& a, uint32_t kl, int rows, int buffers, int next, int wave) const {
         if (a.dim == DP) return;
+        for (int b = 0; b < buffers; ++b)
 #pragma unroll
-        for (int j = 0; j < NI; ++j)
-            if (!(in_head[j % NM] >> (threadIdx.x & 63) & 1)) {
-                const uint32_t at = kl + (wave * NI + j) * 1024 + (threadIdx.x & 63) * 16;
-                *(__attribute__((address_space(3))) u32x4*)(uintptr_t)at = (u32x4)(0u);
-                *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(at + next) = (u32x4)(0u);
-            }
+            for (int j = 0; j < NI; ++j)
+                if ((wave * NI + j) * RPI < rows && !in_head(a, j)) *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(kl + b * next + (wave * NI + j) * 1024 + (threadIdx.x & 63) * 16) = (u32x4)(0u);
     }
-    // The wave's rows of V behind the last key, once they have landed: zero (0 times a V that is infinite there would be NaN).
+    // The wave's rows of V behind the last key become zero (0 times a V that is infinite there would be NaN).
     __device__ __forceinline__ void blank_behind(int j0, int lk, uint32_t vl, int wave) const {
-        const int first = lk - j0 > wave * NI * RPI ? lk - j0 : wave * NI * RPI;
-        for (uint32_t at = vl + first * (DP * 2) + (threadIdx.x & 63) * 16; at < vl + (wave + 1) * NI * 1024; at += 1024) *(__attribute__((address_space(3))) u32x4*)(uintptr_t)at = (u32x4)(0u);
+        const int rows = lk - j0 - wave * NI * RPI, from = rows < 0 ? 0 : rows, lane = threadIdx.x & 63;  // rows of the wave that hold keys
+        uint32_t at = vl + (wave * NI + from / RPI) * 1024 + lane * 16;
+        if (from < NI * RPI && lane / PPR >= from % RPI) *(__attribute__((address_space(3))) u32x4*)(uintptr_t)at = (u32x4)(0u);
+        for (int j = from / RPI + 1; j < NI; ++j) *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(at += 1024) = (u32x4)(0u);
     }
-    // Rows j0 .. of K and V to LDS; rows behind the last key repeat it, so what stands there is never read.
-    template <typename T>
+    // Rows j0 .. of K and V to LDS.  What stands behind the last key is never read: rows there repeat it, or (ZERO) those of V
+    // are zero and not fetched.  (Some instructions then fetch nothing, so a wave that counts its requests blanks them once
+    // they have landed instead.)  Whole tiles have a path of their own: single tokens over long keys gain 11 %.
+    template <bool ZERO, typename T>
     __device__ __forceinline__ void issue(const AttnArgs& a, const T* k, const T* v, int j0, int lk, uint32_t kl, uint32_t vl, int wave) {
         const char* kb = uniform_ptr(k + j0 * a.k_st);
         const char* vb = uniform_ptr(v + j0 * a.v_st);
         const bool whole = j0 + KT <= lk;
         const int behind = row0 - (lk - 1 - j0);  // rows from the last key to row0
         auto back = [&](int j) __attribute__((always_inline)) { return behind + j * RPI > 0 ? behind + j * RPI : 0; };
-        if (a.dim == DP) {
+        if (whole) {
+            if (a.dim == DP) {
 #pragma unroll
-            for (int j = 0; j < NI; ++j) glds16_asm(kb, whole ? kof[j] : kof[j] - back(j) * (int)(a.k_st * 2), kl + (wave * NI + j) * 1024);
+                for (int j = 0; j < NI; ++j) glds16_asm(kb, kof[j], kl + (wave * NI + j) * 1024);
+            } else {
+#pragma unroll
+                for (int j = 0; j < NI; ++j) glds16_masked_asm(kb, kof[j], kl + (wave * NI + j) * 1024, __ballot(in_head(a, j)));
+            }
+#pragma unroll
+            for (int j = 0; j < NI; ++j) glds16_asm(vb, vof[j], vl + (wave * NI + j) * 1024);
         } else {
 #pragma unroll
-            for (int j = 0; j < NI; ++j) glds16_masked_asm(kb, whole ? kof[j] : kof[j] - back(j) * (int)(a.k_st * 2), kl + (wave * NI + j) * 1024, in_head[j % NM]);
-        }
+            for (int j = 0; j < NI; ++j) glds16_masked_asm(kb, kof[j] - back(j) * (int)(a.k_st * 2), kl + (wave * NI + j) * 1024, __ballot(in_head(a, j)));
 #pragma unroll
-        for (int j = 0; j < NI; ++j) glds16_asm(vb, whole ? vof[j] : vof[j] - back(j) * (int)(a.v_st * 2), vl + (wave * NI + j) * 1024);
+            for (int j = 0; j < NI; ++j) {
+                if (ZERO)
+                    glds16_masked_asm(vb, vof[j], vl + (wave * NI + j) * 1024, __ballot(behind + j * RPI <= 0));
+                else
+                    glds16_asm(vb, vof[j] - back(j) * (int)(a.v_st * 2), vl + (wave * NI + j) * 1024);
+            }
+            if (ZERO) blank_behind(j0, lk, vl, wave);
+        }
     }
 };
 
@@ -662,14 +676,14 @@ __global__ __launch_bounds__(256, DP <= 64 && !(BIAS == BIAS_SLOPE && !CAP) && C
     TileLoad<DP, KT, 4> load;
     load.open(a, wv);
     const uint32_t l0 = lds_addr_of(lds);
-    load.blank_pads(a, l0, 2 * TILE, wv);
+    load.blank_pads(a, l0, KT, 2, 2 * TILE, wv);
     // keys that any of the workgroup's rows from row0 on sees, in this chunk; the first tile of them is requested at once
     auto begin = [&](int row0) __attribute__((always_inline)) {
         if (row0 >= rows) return 0;
         const int last = row0 + 127 < rows - 1 ? row0 + 127 : rows - 1;
         int need = limit_of(a, dr, token_of(a, last) + dr.lk - dr.lq, prefix);
         if (need > from + a.chunk) need = from + a.chunk;
-        if (from < need) load.issue(a, kbase, vbase, from, dr.lk, l0, l0 + TILE, wv);
+        if (from < need) load.template issue<true>(a, kbase, vbase, from, dr.lk, l0, l0 + TILE, wv);
         return need;
     };
     int need = begin(t0 * 128);
@@ -685,12 +699,8 @@ __global__ __launch_bounds__(256, DP <= 64 && !(BIAS == BIAS_SLOPE && !CAP) && C
         st.open(a, dr, b, hk, prefix, row0 + wv * 32, r, table);
         int buf = 0;
         for (int j0 = from; j0 < need; j0 += KT, buf ^= 1) {
-            if (j0 + KT > dr.lk) {
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                load.blank_behind(j0, dr.lk, l0 + buf * 2 * TILE + TILE, wv);
-            }
             wait_all_barrier();  // the tile has landed; everyone has read the one before
-            if (j0 + KT < need) load.issue(a, kbase, vbase, j0 + KT, dr.lk, l0 + (buf ^ 1) * 2 * TILE, l0 + (buf ^ 1) * 2 * TILE + TILE, wv);
+            if (j0 + KT < need) load.template issue<true>(a, kbase, vbase, j0 + KT, dr.lk, l0 + (buf ^ 1) * 2 * TILE, l0 + (buf ^ 1) * 2 * TILE + TILE, wv);
             if (j0 < st.lim_max) st.tile(a, lds + buf * 2 * TILE, lds + buf * 2 * TILE + TILE, table, j0);
         }
         st.close(r.live);
@@ -746,20 +756,23 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(AttnArgs a) {
         if (need > from + a.chunk) need = from + a.chunk;
         int buf = 0;
         const int first = from + wv * KT;
-        load.blank_pads(a, l0, 2 * TILE, 0);
-        if (first < need) load.issue(a, kbase, vbase, first, dr.lk, l0, l0 + TILE, 0);
+        if (first < need) {
+            const bool more = first + NW * KT < need;
+            load.blank_pads(a, l0, more ? KT : dr.lk - first, more ? 2 : 1, 2 * TILE, 0);
+            load.template issue<false>(a, kbase, vbase, first, dr.lk, l0, l0 + TILE, 0);
+        }
         for (int j0 = first; j0 < need; j0 += NW * KT, buf ^= 1) {
             // this wave's reads of the other buffer are done (the products that needed them are under way)
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             if (j0 + NW * KT < need) {
-                load.issue(a, kbase, vbase, j0 + NW * KT, dr.lk, l0 + (buf ^ 1) * 2 * TILE, l0 + (buf ^ 1) * 2 * TILE + TILE, 0);
+                load.template issue<false>(a, kbase, vbase, j0 + NW * KT, dr.lk, l0 + (buf ^ 1) * 2 * TILE, l0 + (buf ^ 1) * 2 * TILE + TILE, 0);
                 asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * TileLoad<DP, KT, 1>::NI) : "memory");
             } else {
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             }
             if (j0 + KT > dr.lk) {
                 load.blank_behind(j0, dr.lk, l0 + buf * 2 * TILE + TILE, 0);
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                asm volatile("" ::: "memory");  // (a wave's LDS accesses are done in order)
             }
             st.tile(a, mine + buf * 2 * TILE, mine + buf * 2 * TILE + TILE, table, j0);
         }
