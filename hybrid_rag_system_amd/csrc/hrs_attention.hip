@@ -720,8 +720,8 @@ __global__ __launch_bounds__(256, DP <= 64 && !(BIAS == BIAS_SLOPE && !CAP) && C
 // ---- few rows: up to 32 per document and key head --------------------------------------------------------
 // The waves of a workgroup share the keys instead of the rows: wave w takes tiles w, w + NW, .. of 32 keys through an LDS
 // ring of its own, without a barrier, and the waves' sums meet at the end in a fixed order.
-// Bound by HBM: 8 documents of 32768 keys, 8 key heads of 128, 4 query heads each: 202 us, 5.3 TB/s, the rate of a copy;
-// lengths of 1 .. 32768 177 us (4.2 TB/s; the longest document's chunks end last), with a cap and a slope 205 us.
+// Bound by HBM: 8 documents of 32768 keys, 8 key heads of 128, 4 query heads each: 204 us, 5.2 TB/s, the rate of a copy;
+// lengths of 1 .. 32768 164 us (4.5 TB/s; the longest document's chunks end last), with a cap and a slope 183 us.
 template <typename T, int DP, int NW, int BIAS, int CAP, bool FIXED>
 __global__ __launch_bounds__(64 * NW) void k_attend_few(AttnArgs a) {
     constexpr int KT = 32, TILE = KT * DP * 2, ND = DP / 32, RING = 4 * TILE;
@@ -1028,8 +1028,8 @@ static AttnPlan plan_attention(hrs_ctx* ctx, const hrs_attention_args* p, AttnAr
     }
     // Too few workgroups for the card: long documents are cut into chunks of keys, joined by a second launch.  Few rows
     // (one workgroup fills a CU): two per CU, of 1024 keys at least; more chunks only add to the join.  8 documents of
-    // up to 32768 keys, 8 key heads of 128: 173 us with 4 chunks, 171 with 8, 187 with 16, 220 with 32; one document: 34.6
-    // with 32 chunks, 41.9 with 64.
+    // up to 32768 keys, 8 key heads of 128: 151 us with 4 chunks, 164 with 8, 183 with 16, 215 with 32; 13 documents: 382 with
+    // 2, 373 with 4, 380 with 9, and of 32768 keys each 595, 473, 480.
     const int64_t groups = pairs * (plan.few ? 1 : a.tiles), cus = ctx->num_cu;
     if (groups < 2 * cus && longest_k > 1024) {
         int64_t chunks = (plan.few ? 2 : 4) * cus / groups, most = longest_k / (plan.few ? 1024 : 512);
